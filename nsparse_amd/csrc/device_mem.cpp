@@ -249,21 +249,8 @@ Context &ctx()
     Context &c = per_dev[dev];
     std::lock_guard<std::mutex> lk(mu);
     if (!c.ready) {
-        // the streams of the big-LDS bins (hash bin 4, heavy bin 5, bit-window bin 10) get the highest
-        // priority: their few, large workgroups should take CUs as they free up instead of queueing behind a
-        // million small rows and running alone at the end (NSPARSE_STREAM_PRIO=0: all equal)
-        int prio_lo = 0, prio_hi = 0;
-        (void)hipDeviceGetStreamPriorityRange(&prio_lo, &prio_hi);
-        const bool prio_on = exp_env("NSPARSE_STREAM_PRIO", 1) != 0;
+        // every stream has the default priority: work on streams of different priorities has hung on this part
         for (int i = 0; i < kMaxBins; i++) {
-            // NSPARSE_PRIO_BINS=<bit mask of bins>: which bins' streams get it (default: 4, 5, 10)
-            static const unsigned prio_mask = (unsigned)exp_env("NSPARSE_PRIO_BINS", 0x430);
-            const bool big = prio_on && ((prio_mask >> i) & 1u);
-            if (big) {
-                NSP_CHECK(hipStreamCreateWithPriority(&c.stream[i], hipStreamNonBlocking, prio_hi));
-                NSP_CHECK(hipEventCreateWithFlags(&c.ev_join[i], hipEventDisableTiming));
-                continue;
-            }
             NSP_CHECK(hipStreamCreateWithFlags(&c.stream[i], hipStreamNonBlocking));
             NSP_CHECK(hipEventCreateWithFlags(&c.ev_join[i], hipEventDisableTiming));
         }
