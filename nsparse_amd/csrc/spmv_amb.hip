@@ -434,15 +434,23 @@ static void launch_bs(real *d_y, const sfAMB *mat, const real *d_x, int tb, hipS
 #undef NSP_PIPE
 }
 
+// y = 0 by a kernel: a memset node in a captured graph has given wrong results on replays after the first
+__global__ void k_fill_zero(real *y, int n)
+{
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < n) y[i] = (real)0;
+}
+
 static void launch(real *d_y, const sfAMB *mat, const real *d_x, const sfPlan *plan, hipStream_t st)
 {
     // y = 0 (kernel_spmv_init_ans): needed when the kernel adds into y (several segments) or when
     // all-empty chunks were dropped (their rows are never visited).  With one segment and every
-    // chunk present each row is stored exactly once, and the memset -- a third of the time of a
+    // chunk present each row is stored exactly once, and the fill -- a third of the time of a
     // cache-resident SpMV -- is skipped.
     const bool every_row_stored = mat->seg_num == 1 && (long long)mat->c_size * mat->chunk >= (long long)mat->pad_M;
     static const int no_memset = exp_env("NSPARSE_SPMV_ABL", 0) & 4;  // diagnostics
-    if (!every_row_stored && mat->M > 0 && !no_memset) NSP_CHECK(hipMemsetAsync(d_y, 0, sizeof(real) * (size_t)mat->M, st));
+    if (!every_row_stored && mat->M > 0 && !no_memset)
+        hipLaunchKernelGGL(k_fill_zero, dim3(ceil_div(mat->M, 256)), dim3(256), 0, st, d_y, mat->M);
     if (mat->c_size <= 0) return;
     int tb = (int)plan->thread_block;
     if (tb < 64 || tb > 1024 || (tb & 63)) tb = 256;
