@@ -22,7 +22,7 @@ def unit_resources(prec, unit, extra=()):
     """[{name (demangled), own, vgpr, agpr, sgpr, scratch, occ, lds, vspill, sspill}] of one unit's device code."""
     src = os.path.join(ROOT, "nsparse_amd", "csrc")
     cmd = ["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", '-DNSPARSE_SRC_HASH="x"',
-           "-munsafe-fp-atomics", "-I" + os.path.join(ROOT, "include"), "-I" + src,
+           "-munsafe-fp-atomics", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I" + os.path.join(ROOT, "include"), "-I" + src,
            "-DDOUBLE" if prec == "d" else "-DFLOAT", *extra, "--cuda-device-only", "-c", os.path.join(src, unit + ".hip"),
            "-o", "/dev/null", "-Rpass-analysis=kernel-resource-usage"]
     p = subprocess.run(cmd, capture_output=True, text=True)
