@@ -144,6 +144,36 @@ DIST_SIGNATURES = {
 }
 DIST_ID_BYTES = 128
 
+
+class LmAttn(C.Structure):
+    """nsparse_lm_attn of include/nsparse_lm.h"""
+    _fields_ = [(n, C.c_int) for n in ("dtype", "heads", "kv_heads", "head_dim", "block", "width", "causal", "n_seq", "page_size", "first",
+                                       "local")] + \
+               [("scale", C.c_float), ("q_rows", C.c_longlong), ("k_rows", C.c_longlong), ("table_stride", C.c_longlong)] + \
+               [(n, C.c_void_p) for n in ("cu_q", "cu_k", "q_len", "k_len", "page_table")] + \
+               [("q_stride", C.c_longlong * 2), ("k_stride", C.c_longlong * 3), ("v_stride", C.c_longlong * 3)]
+
+
+# every entry point declared in include/nsparse_lm.h (libnsparse_lm.so: sparse products of language models; nsparse_amd/lm.py is
+# the view of it on torch tensors)
+_V, _L, _I = C.c_void_p, C.c_longlong, C.c_int
+LM_SIGNATURES = {
+    "nsparse_lm_last_error": (_I, []),
+    "nsparse_lm_last_error_string": (C.c_char_p, []),
+    "nsparse_lm_build_info": (C.c_char_p, []),
+    "nsparse_lm_mean_rows": (_L, [_P(LmAttn)]),
+    "nsparse_lm_block_means": (_I, [_P(LmAttn), _V, _V, _I, _V]),
+    "nsparse_lm_select_blocks": (_I, [_P(LmAttn), _V, _V, _V, _V]),
+    "nsparse_lm_block_attention": (_I, [_P(LmAttn)] + [_V] * 7),
+    "nsparse_lm_block_attention_bwd_workspace": (_L, [_P(LmAttn)]),
+    "nsparse_lm_block_attention_bwd": (_I, [_P(LmAttn)] + [_V] * 11 + [_L, _V]),
+    "nsparse_lm_route_workspace": (_L, [_L, _I, _I]),
+    "nsparse_lm_route": (_I, [_V, _L, _I, _I, _V, _V, _V, _V, _L, _V]),
+    "nsparse_lm_gather_tokens": (_I, [_I, _V, _V, _L, _I, _I, _V, _V]),
+    "nsparse_lm_combine_tokens": (_I, [_I, _V, _V, _V, _L, _I, _I, _V, _V]),
+    "nsparse_lm_combine_tokens_bwd": (_I, [_I, _V, _V, _V, _V, _L, _I, _I, _V, _V, _V]),
+}
+
 _libs = {}
 _vendor = {}
 _dist = {}
@@ -297,6 +327,31 @@ class DistLib:
                                               cuts.ctypes.data_as(c_int_p))
         assert rc == 0, rc
         return cuts
+
+
+class LmLib:
+    """libnsparse_lm.so: sparse products whose pattern a language model chooses (include/nsparse_lm.h)."""
+
+    def __init__(self):
+        path = os.path.join(LIB_DIR, "libnsparse_lm.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing: build it with `make -C nsparse_amd/csrc lm`.  There is no fallback path.")
+        self.path = path
+        self.dll = C.CDLL(path, mode=C.RTLD_LOCAL)
+        for name, (res, args) in LM_SIGNATURES.items():
+            fn = getattr(self.dll, name)
+            fn.restype = res
+            fn.argtypes = args
+            setattr(self, name, fn)
+
+
+_lm = []
+
+
+def load_lm():
+    if not _lm:
+        _lm.append(LmLib())
+    return _lm[0]
 
 
 def load_dist(precision="d"):
