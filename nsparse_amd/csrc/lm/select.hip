@@ -66,79 +66,90 @@ __global__ void __launch_bounds__(256) k_block_means(const Geometry G, const T *
 }
 
 // ---- selection ---------------------------------------------------------------------------------------------------------------
-// One workgroup per (query row, key head): the scores of `kScores` blocks at a time in LDS beside the best so far, the best of
-// both by repeated search.
-constexpr int kScores = 4096, kWidest = 256;
+// Scores are computed in 32 bits with a bound of their error,
+//   |score32 - score| <= off = (D + group + 8) 2^-24 |sum_h |q_h|| max_b |mean_b|      (Cauchy-Schwarz over the products),
+// and the need-th best 32-bit score a is found by bisection.  A block above a + 2 off is among the best whatever the errors
+// are, one below a - 2 off is not; what lies between is scored again in 64 bits, wavefront by block, if not all of it is wanted.
+// Rows whose bound is no finite number (NaN, infinities, overflow) or whose band is wide (many equal scores) take the plain way:
+// every score in 64 bits and a search per selected block.
+constexpr int kWidest = 256;
 
-template <class T>
-__global__ void __launch_bounds__(256)
-    k_select(const Geometry G, int first, int local, const T *__restrict__ q, const T *__restrict__ means, int *__restrict__ idx)
+struct Competition {  // the blocks lo .. hi - 1 compete for `need` places
+    int eligible, lo, hi, need;
+};
+__device__ inline Competition competition(const Geometry &G, const Seq &sq, int i, int first, int local)
 {
-    __shared__ double qsum[256];
-    __shared__ double score[kScores + kWidest];
-    __shared__ int name[kScores + kWidest];
-    __shared__ double wave_best[4];
-    __shared__ int wave_at[4];
-    __shared__ double best_score[kWidest];
-    __shared__ int best_name[kWidest];
-    const int g = (int)(blockIdx.x % G.kv_heads), t = (int)(blockIdx.x / G.kv_heads);
-    const int tid = threadIdx.x;
-    Seq sq;
-    const int i = seq_of_query(G, t, sq);
-    if (i < 0) return;
-    int eligible;  // blocks 0 .. eligible - 1
+    Competition c;
     if (G.causal) {
         const int pos = sq.k_len - sq.q_len + i;
-        eligible = pos < 0 ? 0 : pos / G.block + 1;
+        c.eligible = pos < 0 ? 0 : pos / G.block + 1;
     } else {
-        eligible = (sq.k_len + G.block - 1) / G.block;
+        c.eligible = (sq.k_len + G.block - 1) / G.block;
     }
-    int *row = idx + ((long long)t * G.kv_heads + g) * G.width;
-    if (eligible <= G.width) {
-        for (int x = tid; x < G.width; x += 256) row[x] = x < eligible ? x : -1;
-        return;
+    c.lo = first;
+    c.hi = c.eligible > G.width ? c.eligible - local : 0;
+    c.need = G.width - first - local;
+    return c;
+}
+// first element of a block's mean for key head g; NULL where the page table names no page
+template <class T> __device__ inline const T *mean_of_block(const Geometry &G, const Seq &sq, const T *means, int g, int b)
+{
+    long long m;
+    if (G.page_size > 0) {
+        const long long page = page_of_block(G, sq.s, b);
+        if (page < 0) return nullptr;
+        m = page * G.per_page + b % G.per_page;
+    } else {
+        m = mean_base(G, sq) + b;
     }
-    const int lo = first, hi = eligible - local;  // the blocks that compete; eligible > width >= first + local
-    const int need = G.width - first - local;
-    for (int d = tid; d < G.head_dim; d += 256) {
+    return means + (m * G.kv_heads + g) * G.head_dim;
+}
+
+// The plain way, by a whole workgroup: `cap` scores at a time beside the best so far.
+struct Plain {
+    double best_score[kWidest], qsum[256];
+    int wave_at[16], best_name[kWidest];
+};
+template <class T>
+__device__ void select_plain(const Geometry &G, const Seq &sq, int t, int g, const Competition &c, const T *q, const T *means, int *row,
+                             Plain &pl, char *space, int bytes)
+{
+    const int tid = threadIdx.x, threads = blockDim.x;
+    const int slots = bytes / 12, cap = slots - kWidest;
+    double *score = (double *)space;
+    int *name = (int *)(space + 8 * (size_t)slots);
+    __syncthreads();
+    for (int d = tid; d < G.head_dim; d += threads) {
         double s = 0;
         for (int h = 0; h < G.group; h++) s += (double)to_f32(q[(long long)t * G.q_row + (long long)(g * G.group + h) * G.q_head + d]);
-        qsum[d] = s;
+        pl.qsum[d] = s;
     }
     __syncthreads();
     int have = 0;
-    for (int c0 = lo; c0 < hi && need > 0; c0 += kScores) {
-        const int n = hi - c0 < kScores ? hi - c0 : kScores;
-        for (int x = tid; x < have; x += 256) {
-            score[x] = best_score[x];
-            name[x] = best_name[x];
+    for (int c0 = c.lo; c0 < c.hi && c.need > 0; c0 += cap) {
+        const int n = c.hi - c0 < cap ? c.hi - c0 : cap;
+        for (int x = tid; x < have; x += threads) {
+            score[x] = pl.best_score[x];
+            name[x] = pl.best_name[x];
         }
-        for (int x = tid; x < n; x += 256) {
-            const int b = c0 + x;
-            long long m;
-            if (G.page_size > 0) {
-                const long long page = page_of_block(G, sq.s, b);
-                m = page < 0 ? -1 : page * G.per_page + b % G.per_page;
-            } else {
-                m = mean_base(G, sq) + b;
-            }
+        for (int x = tid; x < n; x += threads) {
+            const T *p = mean_of_block(G, sq, means, g, c0 + x);
             double s = -INFINITY;
-            if (m >= 0) {
-                const T *p = means + (m * G.kv_heads + g) * G.head_dim;
+            if (p) {
                 s = 0;
-                for (int d = 0; d < G.head_dim; d++) s += qsum[d] * (double)to_f32(p[d]);
+                for (int d = 0; d < G.head_dim; d++) s += pl.qsum[d] * (double)to_f32(p[d]);
                 if (s != s) s = -INFINITY;
             }
             score[have + x] = s;
-            name[have + x] = b;
+            name[have + x] = c0 + x;
         }
         __syncthreads();
         const int total = have + n;
-        const int take = need < total ? need : total;
+        const int take = c.need < total ? c.need : total;
         for (int r = 0; r < take; r++) {
             double bs = -INFINITY;
             int bn = 0x7fffffff, at = -1;
-            for (int x = tid; x < total; x += 256)
+            for (int x = tid; x < total; x += threads)
                 if (name[x] >= 0 && (score[x] > bs || (score[x] == bs && name[x] < bn))) {
                     bs = score[x];
                     bn = name[x];
@@ -153,32 +164,400 @@ __global__ void __launch_bounds__(256)
                     at = oa;
                 }
             }
-            if ((tid & 63) == 0) {
-                wave_best[tid >> 6] = bs;
-                wave_at[tid >> 6] = at;
-            }
+            if ((tid & 63) == 0) pl.wave_at[tid >> 6] = at;
             __syncthreads();
             if (tid == 0) {
                 int pick = -1;
-                for (int w = 0; w < 4; w++) {
-                    const int a = wave_at[w];
+                for (int w = 0; w < threads >> 6; w++) {
+                    const int a = pl.wave_at[w];
                     if (a < 0) continue;
-                    if (pick < 0 || wave_best[w] > score[pick] || (wave_best[w] == score[pick] && name[a] < name[pick])) pick = a;
+                    if (pick < 0 || score[a] > score[pick] || (score[a] == score[pick] && name[a] < name[pick])) pick = a;
                 }
-                best_score[r] = score[pick];
-                best_name[r] = name[pick];
+                pl.best_score[r] = score[pick];
+                pl.best_name[r] = name[pick];
                 name[pick] = -1;
             }
             __syncthreads();
         }
         have = take;
     }
-    for (int x = tid; x < first; x += 256) row[x] = x;
-    for (int x = tid; x < local; x += 256) row[G.width - local + x] = hi + x;
-    for (int x = tid; x < have; x += 256) {
+    for (int x = tid; x < have; x += threads) {
         int r = 0;
-        for (int y = 0; y < have; y++) r += best_name[y] < best_name[x];
-        row[first + r] = best_name[x];
+        for (int y = 0; y < have; y++) r += pl.best_name[y] < pl.best_name[x];
+        row[c.lo + r] = pl.best_name[x];
+    }
+    __syncthreads();
+}
+
+// The places that no score decides.  Returns whether a competition is left.
+__device__ inline bool write_forced(const Geometry &G, const Competition &c, int first, int local, int *row, int lane, int lanes)
+{
+    if (c.eligible <= G.width) {
+        for (int x = lane; x < G.width; x += lanes) row[x] = x < c.eligible ? x : -1;
+        return false;
+    }
+    for (int x = lane; x < first; x += lanes) row[x] = x;
+    for (int x = lane; x < local; x += lanes) row[G.width - local + x] = c.hi + x;
+    return c.need > 0;
+}
+
+__device__ inline unsigned order_key(float x)
+{
+    const unsigned u = __float_as_uint(x);
+    return (u >> 31) ? ~u : u | 0x80000000u;
+}
+__device__ inline float key_value(unsigned k) { return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k); }
+
+// One wavefront: the best c.need of score[c.lo .. c.hi) (LDS, finite), each off by at most `off`; false: take the plain way.
+template <class T>
+__device__ bool select_wave(const Geometry &G, const Seq &sq, int t, int g, const Competition &c, const T *q, const T *means, float off,
+                            float *score, int *row)
+{
+    const int lane = lane_id();
+    // 2 off, rounded up through the additions below
+    const float band = 2.0f * off;
+    if (!(band < 1e30f)) return false;
+    float lo = INFINITY, hi = -INFINITY;
+    for (int x = c.lo + lane; x < c.hi; x += 64) {
+        const float s = score[x];
+        lo = fminf(lo, s);
+        hi = fmaxf(hi, s);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        lo = fminf(lo, __shfl_xor(lo, d));
+        hi = fmaxf(hi, __shfl_xor(hi, d));
+    }
+    // count(>= key_lo) >= need, count(>= key_hi) < need; by value while that halves well, then by the numbers' bits
+    unsigned key_lo = order_key(lo), key_hi = order_key(hi) + 1;
+    float a = lo;
+    for (int step = 0; key_hi - key_lo > 1; step++) {
+        unsigned key = key_lo + (key_hi - key_lo) / 2;
+        if (step < 14) {
+            const float mid = 0.5f * key_value(key_lo) + 0.5f * key_value(key_hi - 1);
+            const unsigned k = order_key(mid);
+            if (k > key_lo && k < key_hi) key = k;
+        }
+        const float mid = key_value(key);
+        int n = 0;
+        for (int x = c.lo; x < c.hi; x += 64) n += __popcll(__ballot(x + lane < c.hi && score[x + lane] >= mid));
+        if (n >= c.need) key_lo = key; else key_hi = key;
+        if (n == c.need) break;
+    }
+    {
+        // a: the need-th best
+        const float at_least = key_value(key_lo);
+        a = INFINITY;
+        for (int x = c.lo + lane; x < c.hi; x += 64)
+            if (score[x] >= at_least) a = fminf(a, score[x]);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) a = fminf(a, __shfl_xor(a, d));
+    }
+    const float slack = band + 4.0f * 5.9604645e-8f * (fabsf(a) + band);
+    const float above = a + slack, below = a - slack;
+    int sure = 0, between = 0;
+    for (int x = c.lo; x < c.hi; x += 64) {
+        const float s = x + lane < c.hi ? score[x + lane] : -INFINITY;
+        sure += __popcll(__ballot(s > above));
+        between += __popcll(__ballot(s >= below && s <= above));
+    }
+    const int places = c.need - sure;
+    if (between != places) {
+        if (between > 64) return false;
+        double mine[4];  // the group's summed queries at columns lane, lane + 64, ...
+        for (int z = 0; z < 4; z++) {
+            const int d = lane + 64 * z;
+            mine[z] = 0;
+            if (d < G.head_dim)
+                for (int h = 0; h < G.group; h++) mine[z] += (double)to_f32(q[(long long)t * G.q_row + (long long)(g * G.group + h) * G.q_head + d]);
+        }
+        double es = 0;
+        int eb = -1, k = 0;
+        for (int x0 = c.lo; x0 < c.hi; x0 += 64) {
+            const float s = x0 + lane < c.hi ? score[x0 + lane] : -INFINITY;
+            unsigned long long m = __ballot(s >= below && s <= above);
+            while (m) {
+                const int b = x0 + __builtin_ctzll(m);
+                m &= m - 1;
+                const T *p = mean_of_block(G, sq, means, g, b);
+                double e = 0;
+                for (int z = 0; z < 4; z++) {
+                    const int d = lane + 64 * z;
+                    if (d < G.head_dim && p) e += mine[z] * (double)to_f32(p[d]);
+                }
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) e += __shfl_xor(e, d);
+                if (lane == k) {
+                    es = e;
+                    eb = b;
+                }
+                k++;
+            }
+        }
+        int better = 0;
+        for (int y = 0; y < k; y++) {
+            const double os = __shfl(es, y);
+            const int ob = __shfl(eb, y);
+            better += os > es || (os == es && ob < eb);
+        }
+        if (eb >= 0) score[eb] = better < places ? INFINITY : -INFINITY;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    int at = c.lo;
+    for (int x = c.lo; x < c.hi; x += 64) {
+        const bool in = x + lane < c.hi && score[x + lane] >= below;
+        const unsigned long long m = __ballot(in);
+        if (in) row[at + __popcll(m & ((1ULL << lane) - 1))] = x + lane;
+        at += __popcll(m);
+    }
+    return true;
+}
+
+// The bound of a row's scores from the norms; not finite where the scores may not be.  The squares' 1e-30 stands for what underflows:
+// numbers whose square is lost, and products below the smallest normal number (at most head_dim 2^-126 in all).
+__device__ inline float score_off(const Geometry &G, float q_norm2, float mean_norm2)
+{
+    return (G.head_dim + G.group + 8) * 5.9604645e-8f * 1.01f * sqrtf(q_norm2 + 1e-30f) * sqrtf(mean_norm2 + 1e-30f);
+}
+__device__ inline float max_or_nan(float a, float b) { return (b > a || b != b) ? b : a; }
+
+// Prompts: one workgroup per (16 query rows, key head).  The rows' summed queries are the right operand, sixteen block means the left,
+// as 32-bit matrix products; the four wavefronts take every fourth tile of blocks, then four rows each for the
+// choice.  The scores stay in LDS (CAP blocks a row).
+template <class T, int KS, int CAP>
+__global__ void __launch_bounds__(256)
+    k_select_rows(const Geometry G, int first, int local, const T *__restrict__ q, const T *__restrict__ means, int *__restrict__ idx)
+{
+    constexpr int LQ = 32 * KS + 4, LS = CAP + 4;
+    __shared__ float qs[16 * LQ];
+    __shared__ __align__(16) float score[16 * LS];
+    __shared__ float q_norm2[16], mean_norm2[16];  // of the wavefront
+    __shared__ int plain_row[16];
+    __shared__ Plain pl;
+    const int lane = lane_id(), col = lane & 15, quad = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int g = (int)(blockIdx.x % G.kv_heads);
+    const int t0 = (int)(blockIdx.x / G.kv_heads) * 16;
+    const int t1 = t0 + 16 < G.q_rows ? t0 + 16 : G.q_rows;
+    if (threadIdx.x < 16) plain_row[threadIdx.x] = 0;
+    // the group's summed queries, and the norm of the sum of their absolute values
+    {
+        const int r = (int)threadIdx.x >> 4, l16 = (int)threadIdx.x & 15;
+        float n2 = 0.f;
+        for (int d0 = l16 * 8; d0 < 32 * KS; d0 += 128) {
+            float s[8] = {}, n[8] = {};
+            if (t0 + r < t1 && d0 < G.head_dim)
+                for (int h = 0; h < G.group; h++) {
+                    typedef __attribute__((ext_vector_type(8))) T T8;
+                    const T8 x = __builtin_bit_cast(T8, frag_load(q + (long long)(t0 + r) * G.q_row + (long long)(g * G.group + h) * G.q_head + d0));
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        s[i] += (float)x[i];
+                        n[i] += fabsf((float)x[i]);
+                    }
+                }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                qs[r * LQ + d0 + i] = s[i];
+                n2 += n[i] * n[i];
+            }
+        }
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) n2 += __shfl_xor(n2, d);
+        if (l16 == 0) q_norm2[r] = n2;
+    }
+    __syncthreads();
+    Frag<float> qf[KS];
+#pragma unroll
+    for (int z = 0; z < KS; z++) {
+        const float *p = qs + col * LQ + 32 * z + 8 * quad;
+        qf[z] = frag_load(p);
+    }
+    // the rows may belong to several sequences: one after the other
+    for (int a = t0; a < t1;) {
+        Seq sq;
+        const int i0 = seq_of_query(G, a, sq);
+        if (i0 < 0) {
+            a++;
+            continue;
+        }
+        const int z = sq.q_base + sq.q_len < t1 ? (int)(sq.q_base + sq.q_len) : t1;
+        const int hi = competition(G, sq, (int)(z - 1 - sq.q_base), first, local).hi;  // the last row's is the greatest
+        float n2max = 0.f;
+        for (int b0 = first / 16 * 16 + 16 * wave; b0 < hi; b0 += 64) {
+            const int b = b0 + col;
+            const T *p = b < hi ? mean_of_block(G, sq, means, g, b) : nullptr;
+            const bool hidden = b < hi && !p;
+            f32x4 s = f32x4{0, 0, 0, 0};
+            float n2 = 0.f;
+#pragma unroll
+            for (int x = 0; x < KS; x++) {
+                const int d = 32 * x + 8 * quad;
+                typedef __attribute__((ext_vector_type(8))) T T8;
+                T8 v{};
+                if (p && d < G.head_dim) v = __builtin_bit_cast(T8, frag_load(p + d));
+                Frag<float> f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    f.lo[i] = (float)v[i];
+                    f.hi[i] = (float)v[4 + i];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) n2 += f.lo[i] * f.lo[i] + f.hi[i] * f.hi[i];
+                s = mma(f, qf[x], s);
+            }
+            // a block whose page is none scores lowest: the plain way sees to that
+            n2max = max_or_nan(n2max, hidden ? NAN : quads_sum(n2));
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (b0 + 4 * quad + i < hi && t0 + col >= a && t0 + col < z) score[col * LS + b0 + 4 * quad + i] = s[i];
+        }
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) n2max = max_or_nan(n2max, __shfl_xor(n2max, d));
+        if (lane == 0) mean_norm2[wave] = n2max;
+        __syncthreads();
+        const float m2 = max_or_nan(max_or_nan(mean_norm2[0], mean_norm2[1]), max_or_nan(mean_norm2[2], mean_norm2[3]));
+        for (int t = a + ((wave - (a - t0)) & 3); t < z; t += 4) {
+            const Competition c = competition(G, sq, (int)(t - sq.q_base), first, local);
+            int *row = idx + ((long long)t * G.kv_heads + g) * G.width;
+            if (!write_forced(G, c, first, local, row, lane, 64)) continue;
+            if (!select_wave(G, sq, t, g, c, q, means, score_off(G, q_norm2[t - t0], m2), score + (t - t0) * LS, row)) plain_row[t - t0] = 1;
+        }
+        __syncthreads();
+        for (int t = a; t < z; t++)
+            if (plain_row[t - t0])
+                select_plain(G, sq, t, g, competition(G, sq, (int)(t - sq.q_base), first, local), q, means,
+                             idx + ((long long)t * G.kv_heads + g) * G.width, pl, (char *)score, (int)sizeof(score));
+        __syncthreads();
+        a = z;
+    }
+}
+
+// Single tokens: one workgroup per (query row, key head); sixteen lanes share a block's mean.
+constexpr int kOneCap = 32768;
+template <class T>
+__global__ void __launch_bounds__(1024)
+    k_select_one(const Geometry G, int first, int local, const T *__restrict__ q, const T *__restrict__ means, int *__restrict__ idx)
+{
+    extern __shared__ __align__(16) float score[];
+    __shared__ float norms[16];
+    __shared__ int plain;
+    __shared__ Plain pl;
+    const int lane = lane_id(), l16 = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int g = (int)(blockIdx.x % G.kv_heads), t = (int)(blockIdx.x / G.kv_heads);
+    Seq sq;
+    const int i = seq_of_query(G, t, sq);
+    if (i < 0) return;
+    const Competition c = competition(G, sq, i, first, local);
+    int *row = idx + ((long long)t * G.kv_heads + g) * G.width;
+    if (!write_forced(G, c, first, local, row, (int)threadIdx.x, 1024)) return;
+    typedef __attribute__((ext_vector_type(8))) T T8;
+    float s[16] = {}, q2 = 0.f;
+#pragma unroll
+    for (int z = 0; z < 2; z++) {
+        const int d = 128 * z + 8 * l16;
+        float n[8] = {};
+        if (d < G.head_dim)
+            for (int h = 0; h < G.group; h++) {
+                const T8 x = __builtin_bit_cast(T8, frag_load(q + (long long)t * G.q_row + (long long)(g * G.group + h) * G.q_head + d));
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    s[8 * z + e] += (float)x[e];
+                    n[e] += fabsf((float)x[e]);
+                }
+            }
+#pragma unroll
+        for (int e = 0; e < 8; e++) q2 += n[e] * n[e];
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) q2 += __shfl_xor(q2, d);
+    float n2max = 0.f;
+    for (int b = c.lo + (int)(threadIdx.x >> 4); b < c.hi; b += 64) {
+        const T *p = mean_of_block(G, sq, means, g, b);
+        float dot = 0.f, n2 = 0.f;
+#pragma unroll
+        for (int z = 0; z < 2; z++) {
+            const int d = 128 * z + 8 * l16;
+            if (p && d < G.head_dim) {
+                const T8 x = __builtin_bit_cast(T8, frag_load(p + d));
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    dot += s[8 * z + e] * (float)x[e];
+                    n2 += (float)x[e] * (float)x[e];
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) {
+            dot += __shfl_xor(dot, d);
+            n2 += __shfl_xor(n2, d);
+        }
+        n2max = max_or_nan(n2max, p ? n2 : NAN);
+        if (l16 == 0) score[b] = dot;
+    }
+#pragma unroll
+    for (int d = 16; d < 64; d <<= 1) n2max = max_or_nan(n2max, __shfl_xor(n2max, d));
+    if (lane == 0) norms[wave] = n2max;
+    __syncthreads();
+    if (wave == 0) {
+        float m2 = norms[0];
+        for (int w = 1; w < 16; w++) m2 = max_or_nan(m2, norms[w]);
+        const bool done = select_wave(G, sq, t, g, c, q, means, score_off(G, q2, m2), score, row);
+        if (lane == 0) plain = !done;
+    }
+    __syncthreads();
+    if (plain) select_plain(G, sq, t, g, c, q, means, row, pl, (char *)score, 8192 * 4);
+}
+
+// Sequences of more blocks than LDS holds scores for: the plain way for every row.
+template <class T>
+__global__ void __launch_bounds__(256)
+    k_select_long(const Geometry G, int first, int local, const T *__restrict__ q, const T *__restrict__ means, int *__restrict__ idx)
+{
+    __shared__ __align__(16) char space[12 * 4096];
+    __shared__ Plain pl;
+    const int g = (int)(blockIdx.x % G.kv_heads), t = (int)(blockIdx.x / G.kv_heads);
+    Seq sq;
+    const int i = seq_of_query(G, t, sq);
+    if (i < 0) return;
+    const Competition c = competition(G, sq, i, first, local);
+    int *row = idx + ((long long)t * G.kv_heads + g) * G.width;
+    if (write_forced(G, c, first, local, row, (int)threadIdx.x, 256)) select_plain(G, sq, t, g, c, q, means, row, pl, space, (int)sizeof(space));
+}
+
+template <class T, int KS>
+static void launch_rows(const Geometry &G, long long blocks, int first, int local, const void *q, const void *means, int *idx, hipStream_t st)
+{
+    const dim3 grid((unsigned)(ceil_div(G.q_rows, 16) * G.kv_heads));
+    if (blocks <= 256)
+        hipLaunchKernelGGL((k_select_rows<T, KS, 256>), grid, dim3(256), 0, st, G, first, local, (const T *)q, (const T *)means, idx);
+    else if (blocks <= 768)
+        hipLaunchKernelGGL((k_select_rows<T, KS, 768>), grid, dim3(256), 0, st, G, first, local, (const T *)q, (const T *)means, idx);
+    else
+        hipLaunchKernelGGL((k_select_rows<T, KS, 2048>), grid, dim3(256), 0, st, G, first, local, (const T *)q, (const T *)means, idx);
+}
+
+template <class T>
+static void launch_select(const Geometry &G, int first, int local, const void *q, const void *means, int *idx, hipStream_t st)
+{
+    // the most blocks a sequence can have, as far as the host knows
+    const long long blocks = G.page_size > 0 ? G.table_stride * G.per_page : G.cu_k ? ceil_div(G.k_rows, G.block) : G.blocks_each;
+    if (blocks <= 2048 && G.q_rows / G.n_seq >= 4) {
+        if (G.head_dim <= 64) launch_rows<T, 2>(G, blocks, first, local, q, means, idx, st);
+        else if (G.head_dim <= 128) launch_rows<T, 4>(G, blocks, first, local, q, means, idx, st);
+        else launch_rows<T, 8>(G, blocks, first, local, q, means, idx, st);
+        return;
+    }
+    const dim3 grid((unsigned)((long long)G.q_rows * G.kv_heads));
+    if (blocks <= kOneCap) {
+        // the plain way wants 32 KB
+        const size_t lds = blocks <= 8192 ? 8192 * 4 : (size_t)blocks * 4;
+        if (lds > 65536) (void)hipFuncSetAttribute((const void *)k_select_one<T>, hipFuncAttributeMaxDynamicSharedMemorySize, kOneCap * 4);
+        hipLaunchKernelGGL(k_select_one<T>, grid, dim3(1024), lds, st, G, first, local, (const T *)q, (const T *)means, idx);
+    } else {
+        hipLaunchKernelGGL(k_select_long<T>, grid, dim3(256), 0, st, G, first, local, (const T *)q, (const T *)means, idx);
     }
 }
 
@@ -230,14 +609,10 @@ int nsparse_lm_select_blocks(const nsparse_lm_attn *a, const void *q, const void
     if (G.q_rows == 0) return 0;
     if (!q || !idx || (G.k_rows > 0 && !means)) return fail(NSPARSE_LM_EARG, "select_blocks: a required pointer is NULL");
     if (((uintptr_t)q | (uintptr_t)means) & 15) return fail(NSPARSE_LM_EALIGN, "select_blocks: q and means begin at multiples of 16 bytes");
-    const dim3 grid((unsigned)((long long)G.q_rows * G.kv_heads));
     hipStream_t st = (hipStream_t)stream;
-    if (a->dtype == NSPARSE_LM_BF16)
-        hipLaunchKernelGGL(k_select<__bf16>, grid, dim3(256), 0, st, G, a->first, a->local, (const __bf16 *)q, (const __bf16 *)means, idx);
-    else if (a->dtype == NSPARSE_LM_F16)
-        hipLaunchKernelGGL(k_select<_Float16>, grid, dim3(256), 0, st, G, a->first, a->local, (const _Float16 *)q, (const _Float16 *)means, idx);
-    else
-        hipLaunchKernelGGL(k_select<float>, grid, dim3(256), 0, st, G, a->first, a->local, (const float *)q, (const float *)means, idx);
+    if (a->dtype == NSPARSE_LM_BF16) launch_select<__bf16>(G, a->first, a->local, q, means, idx, st);
+    else if (a->dtype == NSPARSE_LM_F16) launch_select<_Float16>(G, a->first, a->local, q, means, idx, st);
+    else launch_select<float>(G, a->first, a->local, q, means, idx, st);
     return launched("select_blocks");
 }
 }
