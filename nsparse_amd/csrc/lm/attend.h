@@ -75,6 +75,55 @@ __device__ inline int visible_keys(const Geometry &G, const Seq &sq, int i)
     return lim < 0 ? 0 : lim;
 }
 
+// ---- several query rows at once -------------------------------------------------------------------------------------------
+// The rows of neighbouring queries list mostly the same blocks.  A wavefront that has several of them walks the union of their
+// rows, block by block upwards: lane i < 32 is a cursor on row i (the entries that count ascend, see the header), the least head is
+// the next block, the lanes whose head it is are the queries that list it.
+struct Cursors {
+    const int *row;
+    int at, width;   // next entry, entries
+    int ahead;       // entry `at`, fetched early
+    int seen, head;  // greatest entry so far; the next that counts, kNone behind the last
+    int blocks;      // blocks with keys that this row's query sees
+};
+constexpr int kNone = 0x7fffffff;
+
+__device__ inline void cursor_advance(Cursors &c)
+{
+    c.head = kNone;
+    while (c.at < c.width) {
+        const int e = c.ahead;
+        if (++c.at < c.width) c.ahead = c.row[c.at];
+        if (e > c.seen) {
+            c.seen = e;
+            if (e < c.blocks) c.head = e; else c.at = c.width;  // all that could count behind it is greater still
+            break;
+        }
+    }
+}
+__device__ inline Cursors cursor_open(const int *row, int width, int blocks, bool live)
+{
+    Cursors c;
+    c.row = row;
+    c.width = (live && blocks > 0) ? width : 0;
+    c.at = 0;
+    c.seen = -1;
+    c.blocks = blocks;
+    c.ahead = c.width > 0 ? row[0] : -1;
+    cursor_advance(c);
+    return c;
+}
+// the next block of the union and the lanes that list it; kNone at the end
+__device__ inline int cursors_next(Cursors &c, unsigned &who)
+{
+    const int b = least_of_32(c.head);
+    const bool mine = c.head == b;
+    who = (unsigned)__ballot(mine);
+    if (b == kNone) return kNone;
+    if (mine) cursor_advance(c);
+    return b;
+}
+
 // a lane's fragments of one row: the chunks of eight columns 32 * s + 8 * quad
 template <class T, int KS, bool FULL> __device__ inline void row_frags(Frag<T> (&f)[KS], const T *p, int quad, int head_dim, bool live)
 {

@@ -199,14 +199,34 @@ __device__ inline long long read_lane64(long long v, int lane)
 // over the four lane groups that share a column of a product's output
 __device__ inline float quads_max(float x)
 {
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ inline float quads_sum(float x)
 {
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+// the least of the first 32 lanes, in a scalar register
+__device__ inline int least_of_32(int x)
+{
+    int o = __builtin_amdgcn_mov_dpp(x, 0xb1, 0xf, 0xf, false);  // neighbours
+    x = o < x ? o : x;
+    o = __builtin_amdgcn_mov_dpp(x, 0x4e, 0xf, 0xf, false);  // pairs
+    x = o < x ? o : x;
+    o = __builtin_amdgcn_mov_dpp(x, 0x141, 0xf, 0xf, false);  // mirrored halves of 16
+    x = o < x ? o : x;
+    o = __builtin_amdgcn_mov_dpp(x, 0x140, 0xf, 0xf, false);  // mirrored 16
+    x = o < x ? o : x;
+    const int a = read_lane(x, 0), b = read_lane(x, 16);
+    return a < b ? a : b;
+}
+// 2^x in one instruction; what is below 2^-126 becomes 0, which no sum next to a 1 can tell
+__device__ inline float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ---- geometry of a call ------------------------------------------------------------------------------------------------
 struct Geometry {
