@@ -76,52 +76,268 @@ __device__ inline int visible_keys(const Geometry &G, const Seq &sq, int i)
 }
 
 // ---- several query rows at once -------------------------------------------------------------------------------------------
-// The rows of neighbouring queries list mostly the same blocks.  A wavefront that has several of them walks the union of their
-// rows, block by block upwards: lane i < 32 is a cursor on row i (the entries that count ascend, see the header), the least head is
-// the next block, the lanes whose head it is are the queries that list it.
-struct Cursors {
-    const int *row;
-    int at, width;   // next entry, entries
-    int ahead;       // entry `at`, fetched early
-    int seen, head;  // greatest entry so far; the next that counts, kNone behind the last
-    int blocks;      // blocks with keys that this row's query sees
+// The rows of neighbouring queries list mostly the same blocks.  A workgroup that has up to 64 of them walks the union of their
+// rows: for a range of blocks, one word a block says which queries list it, and the blocks with a word that is not 0, upwards,
+// are the walk.
+constexpr int kRange = 1024;
+struct Union {
+    unsigned long long who[kRange];
+    unsigned short list[kRange];
+    int n;
 };
-constexpr int kNone = 0x7fffffff;
-
-__device__ inline void cursor_advance(Cursors &c)
+// By a workgroup of four wavefronts: blocks b0 .. b0 + nb of the rows t0 + i, i in `now`; lane i holds row i's visible keys.
+__device__ inline void union_build(Union &u, const Geometry &G, const int *idx, int g, int t0, unsigned long long now, int limit, int b0, int nb,
+                                   int wave)
 {
-    c.head = kNone;
-    while (c.at < c.width) {
-        const int e = c.ahead;
-        if (++c.at < c.width) c.ahead = c.row[c.at];
-        if (e > c.seen) {
-            c.seen = e;
-            if (e < c.blocks) c.head = e; else c.at = c.width;  // all that could count behind it is greater still
-            break;
+    __syncthreads();
+    for (int x = threadIdx.x; x < nb; x += 256) u.who[x] = 0;
+    __syncthreads();
+    if (G.width <= 16) {
+        // four rows at a time, sixteen lanes each; all of them are on their way before the first is looked at
+        const int sub = lane_id() >> 4, j = lane_id() & 15;
+        int e[4];
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+            const int n = 16 * p + 4 * wave + sub;
+            e[p] = ((now >> n) & 1) && j < G.width ? idx[((long long)(t0 + n) * G.kv_heads + g) * G.width + j] : -1;
+        }
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+            const int n = 16 * p + 4 * wave + sub;
+            if (!((now >> (16 * p + 4 * wave)) & 15)) continue;
+            int top = e[p], o;  // greatest entry up to and including this lane's
+            o = __builtin_amdgcn_update_dpp(-1, top, 0x111, 0xf, 0xf, false);
+            top = o > top ? o : top;
+            o = __builtin_amdgcn_update_dpp(-1, top, 0x112, 0xf, 0xf, false);
+            top = o > top ? o : top;
+            o = __builtin_amdgcn_update_dpp(-1, top, 0x114, 0xf, 0xf, false);
+            top = o > top ? o : top;
+            o = __builtin_amdgcn_update_dpp(-1, top, 0x118, 0xf, 0xf, false);
+            top = o > top ? o : top;
+            const int before = __builtin_amdgcn_update_dpp(-1, top, 0x111, 0xf, 0xf, false);
+            const int lim = __shfl(limit, n), b = e[p];
+            if (b > before && (long long)b * G.block < lim && b >= b0 && b < b0 + nb) atomicOr((unsigned *)&u.who[b - b0] + (n >> 5), 1u << (n & 31));
+        }
+    } else {
+        for (int n = wave; n < 64; n += 4) {
+            if (!((now >> n) & 1)) continue;
+            const int lim = read_lane(limit, n);
+            const int *row = idx + ((long long)(t0 + n) * G.kv_heads + g) * G.width;
+            int seen = -1;
+            for (int at = 0; at < G.width; at += 64) {
+                int b;
+                const int c = pattern_chunk(row, at, G.width, (lim + G.block - 1) / G.block, seen, b);
+                if (lane_id() < c && b >= b0 && b < b0 + nb) atomicOr((unsigned *)&u.who[b - b0] + (n >> 5), 1u << (n & 31));
+            }
+        }
+    }
+    __syncthreads();
+    if (wave == 0) {
+        int n = 0;
+        for (int x = 0; x < nb; x += 64) {
+            const bool in = x + lane_id() < nb && u.who[x + lane_id()] != 0;
+            const unsigned long long m = __ballot(in);
+            if (in) u.list[n + __popcll(m & ((1ULL << lane_id()) - 1))] = (unsigned short)(x + lane_id());
+            n += __popcll(m);
+        }
+        if (lane_id() == 0) u.n = n;
+    }
+    __syncthreads();
+}
+
+// NG groups of sixteen keys of a walk.  WIDE: a block has at least as many, they are neighbours; else up to NG blocks.
+template <int NG, bool WIDE> struct Step {
+    static constexpr int kParts = WIDE ? 1 : NG;
+    long long k_off[kParts], v_off[kParts];  // elements from k and v, the head's offset included
+    int from[kParts], left[kParts];          // first key inside the sequence; keys from there on that some listing query sees
+    unsigned long long who[kParts], any;     // queries that list the block
+    __device__ inline int first(int y) const { return WIDE ? from[0] + 16 * y : from[y]; }
+    __device__ inline int rows(int y) const { return WIDE ? left[0] - 16 * y : left[y]; }
+    __device__ inline unsigned long long lists(int y) const { return who[WIDE ? 0 : y]; }
+};
+template <int NG, bool WIDE> __device__ inline int walk_steps(const Geometry &G, const Union &u)
+{
+    const int groups = uniform(u.n) * (G.block >> 4);
+    return (groups + NG - 1) / NG;
+}
+template <int NG, bool WIDE>
+__device__ inline void walk_step(Step<NG, WIDE> &s, const Geometry &G, const Seq &sq, int g, const Union &u, int b0, int limit, int step)
+{
+    const int shift = 27 - __builtin_clz(G.block), groups = uniform(u.n) << shift;
+    s.any = 0;
+#pragma unroll
+    for (int y = 0; y < Step<NG, WIDE>::kParts; y++) {
+        const int i = step * NG + y;
+        s.k_off[y] = (long long)g * G.k_head;
+        s.v_off[y] = (long long)g * G.v_head;
+        s.from[y] = 0;
+        s.left[y] = 0;
+        s.who[y] = 0;
+        if (i >= groups) continue;
+        const int e = uniform(u.list[i >> shift]), b = b0 + e;
+        const unsigned long long who = uniform64(u.who[e]);
+        const int part = i & ((1 << shift) - 1);
+        const int start = b * G.block + part * 16;
+        // the last of the listing rows sees the most
+        int left = read_lane(limit, 63 - __builtin_clzll(who)) - start;
+        const int end = (WIDE ? NG * 16 : 16);
+        long long r = sq.k_base + start, page = 0;
+        if (G.page_size > 0) {
+            page = page_of_block(G, sq.s, b);
+            if (page < 0) left = 0;
+            r = (long long)(b % G.per_page) * G.block + part * 16;
+        }
+        if (left <= 0) continue;
+        s.k_off[y] += page * G.k_page + r * G.k_row;
+        s.v_off[y] += page * G.v_page + r * G.v_row;
+        s.from[y] = start;
+        s.left[y] = left < end ? left : end;
+        s.who[y] = who;
+        s.any |= who;
+    }
+}
+
+// ---- keys and values in LDS ---------------------------------------------------------------------------------------------
+// Rows of DP elements in pieces of 16 bytes; piece c of row r stands at c ^ (r % 16) (modulo the row), so that sixteen rows' equal
+// pieces, which the fragments of a product read, lie in different banks, and a whole row, which the transposing read
+// wants, stays in one stretch.  Columns behind head_dim and keys that nobody sees hold zeros.
+template <class T, int DP> struct Tile {
+    static constexpr int kPieces = DP * (int)sizeof(T) / 16;
+    static constexpr int kSwizzle = kPieces < 16 ? kPieces - 1 : 15;
+    static constexpr int kPer = 16 / (int)sizeof(T);  // elements a piece
+    static __device__ inline int at(int r, int c) { return r * kPieces + (c ^ (r & kSwizzle)); }
+};
+template <class T, int DP> __device__ inline Frag<T> tile_frag(const u32x4 *t, int r, int s, int quad)
+{
+    if constexpr (sizeof(T) == 2) {
+        return Frag<T>{t[Tile<T, DP>::at(r, 4 * s + quad)]};
+    } else {
+        const int c = 8 * s + 2 * quad;
+        return Frag<T>{__builtin_bit_cast(f32x4, t[Tile<T, DP>::at(r, c)]), __builtin_bit_cast(f32x4, t[Tile<T, DP>::at(r, c + 1)])};
+    }
+}
+// A transposed operand: slots 0 .. 3 are rows 4 quad + i of group y, slots 4 .. 7 those of group y + 1.  Sixteen-bit types: the
+// LDS unit transposes 4 rows x 16 columns for sixteen lanes at a time, lane i of them names columns 4 (i % 4) of row i / 4 and gets
+// column i of the four rows; row m of fragment j is column 16 j + m.  Single precision: E neighbouring columns a lane and row, row m of
+// fragment j is column E m + j (as in rows_column).
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+template <class T, int DP> struct Columns {
+    const u32x4 *t;
+    int y;
+    __device__ inline Columns(const u32x4 *tile, int group, int quad, int col) : t(tile), y(group), q(quad), c(col) {}
+    __device__ inline Frag<T> frag(int j) const
+    {
+        const int r = 16 * y + 4 * q + (c >> 2), piece = 2 * j + ((c & 3) >> 1);
+        const u32x4 *p0 = t + Tile<T, DP>::at(r, piece), *p1 = t + Tile<T, DP>::at(r + 16, piece);
+        typedef __attribute__((address_space(3))) s16x4 *lds;
+        const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)((const u32x2 *)p0 + (c & 1))));
+        const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)((const u32x2 *)p1 + (c & 1))));
+        return Frag<T>{u32x4{a[0], a[1], b[0], b[1]}};
+    }
+    // column of output row 4 quad + e of fragment j, and how many fragments' outputs are neighbours
+    static __device__ inline int column(int j, int quad, int e) { return 16 * j + 4 * quad + e; }
+    int q, c;
+};
+template <int DP> struct Columns<float, DP> {
+    static constexpr int E = DP / 16;
+    Rows<float, E> x;
+    __device__ inline Columns(const u32x4 *t, int y, int quad, int col)
+    {
+#pragma unroll
+        for (int s = 0; s < 8; s++)
+#pragma unroll
+            for (int c = 0; c < E / 4; c++) {
+                const u32x4 v = t[Tile<float, DP>::at(16 * (y + (s >> 2)) + 4 * quad + (s & 3), col * (E / 4) + c)];
+#pragma unroll
+                for (int i = 0; i < 4; i++) x.w[s][4 * c + i] = __uint_as_float(v[i]);
+            }
+    }
+    __device__ inline Frag<float> frag(int j) const { return rows_column(x, j); }
+};
+// o[j][e] * f of a product with Columns, to an output row
+template <class T, int DP> __device__ inline void store_row(T *p, const f32x4 (&o)[DP / 16], float f, int quad, int head_dim)
+{
+    constexpr int E = DP / 16;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int j = 0; j < E; j++) {
+            const int d = 16 * j + 4 * quad;
+            if (d < head_dim) *(u32x2 *)(p + d) = u32x2{pack2(o[j][0] * f, o[j][1] * f, T{}), pack2(o[j][2] * f, o[j][3] * f, T{})};
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            float w[E];
+#pragma unroll
+            for (int j = 0; j < E; j++) w[j] = o[j][e] * f;
+            const int d = (4 * quad + e) * E;
+            store_columns<T, E>(p + d, w, head_dim - d);
         }
     }
 }
-__device__ inline Cursors cursor_open(const int *row, int width, int blocks, bool live)
+// A step's keys (or values) to LDS, by 256 threads.  Whole tiles go there straight from memory (the wait is the barrier's); tiles with
+// keys that nobody sees, or rows shorter than DP, through registers, with zeros for what is not there.
+template <class T, int DP, int NG, bool WIDE>
+__device__ inline void tile_load(u32x4 *t, const T *p, const long long (&off)[WIDE ? 1 : NG], const Step<NG, WIDE> &s, long long stride, int head_dim)
 {
-    Cursors c;
-    c.row = row;
-    c.width = (live && blocks > 0) ? width : 0;
-    c.at = 0;
-    c.seen = -1;
-    c.blocks = blocks;
-    c.ahead = c.width > 0 ? row[0] : -1;
-    cursor_advance(c);
-    return c;
+    constexpr int kPieces = Tile<T, DP>::kPieces, kPer = Tile<T, DP>::kPer;
+    constexpr int kRows = 256 / kPieces;  // rows a pass
+    constexpr int kPasses = NG * 16 / kRows;
+    static_assert(kRows <= 16 || kRows % 16 == 0, "a pass covers whole groups or a part of one");
+    const int at = (int)threadIdx.x % kPieces, r0 = (int)threadIdx.x / kPieces;
+    bool whole = head_dim == DP;
+#pragma unroll
+    for (int y = 0; y < NG; y++) whole = whole && s.rows(y) >= 16;
+#pragma unroll
+    for (int i = 0; i < kPasses; i++) {
+        const int r = r0 + i * kRows, y0 = i * kRows / 16;
+        const int c = (at ^ (r & Tile<T, DP>::kSwizzle)) * kPer;
+        long long o;
+        int n;
+        if constexpr (WIDE) {
+            o = off[0] + (long long)r * stride + c;
+            n = s.left[0] - (r & ~15);
+        } else {
+            o = off[y0];
+            n = s.left[y0];
+#pragma unroll
+            for (int z = 1; z < kRows / 16; z++)
+                if (r0 >> 4 == z) {
+                    o = off[y0 + z];
+                    n = s.left[y0 + z];
+                }
+            o += (long long)(r & 15) * stride + c;
+        }
+        if (whole) {
+            // lane i's 16 bytes land at the wavefront's base + 16 i
+            u32x4 *base = t + i * 256 + uniform((int)(threadIdx.x & ~63u));
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(p + o), (__attribute__((address_space(3))) void *)base, 16, 0, 0);
+        } else {
+            u32x4 x = u32x4{0, 0, 0, 0};
+            if ((r & 15) < n && c < head_dim) x = *(const u32x4 *)(p + o);
+            t[i * 256 + threadIdx.x] = x;
+        }
+    }
 }
-// the next block of the union and the lanes that list it; kNone at the end
-__device__ inline int cursors_next(Cursors &c, unsigned &who)
+
+// A run of products whose operands come from LDS: AHEAD operands are on their way before the first product, and the next ones are
+// asked for after every STEP, so that no product waits for the read just before it.  The fences keep the compiler from
+// putting each read back before its use.
+template <class F, int N, int AHEAD, int STEP, class Load, class Use> __device__ inline void pipelined(Load load, Use use)
 {
-    const int b = least_of_32(c.head);
-    const bool mine = c.head == b;
-    who = (unsigned)__ballot(mine);
-    if (b == kNone) return kNone;
-    if (mine) cursor_advance(c);
-    return b;
+    F f[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) f[i] = load(i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < N; i += STEP) {
+#pragma unroll
+        for (int s = 0; s < STEP; s++) use(i + s, f[(i + s) % AHEAD]);
+#pragma unroll
+        for (int s = 0; s < STEP; s++)
+            if (i + s + AHEAD < N) f[(i + s) % AHEAD] = load(i + s + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 // a lane's fragments of one row: the chunks of eight columns 32 * s + 8 * quad

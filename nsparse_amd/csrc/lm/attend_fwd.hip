@@ -7,9 +7,9 @@
 // 4 (l / 16) + i, which, rounded, is already the right operand of O^T = V^T P^T; V is read row by row, E = DP / 16
 // neighbouring columns a lane, and transposed inside the lane (common.h).  The softmax runs over the blocks with
 // a running maximum and sum in 32 bits, in base 2.
-// Prompts: a wavefront takes several neighbouring rows, NT x (16 / heads of the group) of them, as the columns of NT products, and walks the
-// union of their blocks (attend.h), so a block that neighbours share is read once.  K and V come out of the L2 cache at what a compute
-// unit's vector memory path carries, and that bound is per block read: the fewer reads a row, the better.
+// Prompts: a workgroup takes several neighbouring rows, 4 NT x (16 / heads of the group) of them, as the columns of the products of its
+// four wavefronts, and walks the union of their blocks (attend.h): a block that neighbours share is read from the L2 cache
+// once, into LDS, while the block before is computed.
 // With few rows (a serving step) eight wavefronts share a row: wavefront w takes every eighth tile of keys and the partial
 // results meet in LDS.
 #include "attend.h"
@@ -166,30 +166,29 @@ __global__ void __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256)
 }
 
 // ---- prompts ---------------------------------------------------------------------------------------------------------------
-template <class T, int DP, int NT, int NG, bool FULL>
-__global__ void __launch_bounds__(256, NT > 1 ? 2 : 1)
+template <class T, int DP, int NT, int NG, bool WIDE>
+__global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
     k_attend_tiles(const Geometry G, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ idx,
                    T *__restrict__ out, float *__restrict__ lse, int slices, int per_tile)
 {
-    constexpr int KS = DP / 32, E = DP / 16;
+    constexpr int KS = DP / 32, E = DP / 16, kTile = NG * 16 * Tile<T, DP>::kPieces;
+    __shared__ u32x4 kt[2][kTile], vt[2][kTile];
+    __shared__ Union un;
     const int lane = lane_id(), col = lane & 15, quad = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int wave = uniform((int)(threadIdx.x >> 6));
+    // consecutive workgroups go round the key heads: with 8 of them each XCD's cache serves one head's keys
     const int g = (int)(blockIdx.x % G.kv_heads);
     const int rest = (int)(blockIdx.x / G.kv_heads);
     const int slice = rest % slices;
     const int per_wave = NT * per_tile;  // rows a wavefront
-    const int t0 = ((rest / slices) * 4 + wave) * per_wave;
-    if (t0 >= G.q_rows) return;
-    const int t1 = t0 + per_wave < G.q_rows ? t0 + per_wave : G.q_rows;
+    const int t0 = (rest / slices) * 4 * per_wave;
+    const int t1 = t0 + 4 * per_wave < G.q_rows ? t0 + 4 * per_wave : G.q_rows;
     const int D = G.head_dim;
     const int heads = G.group < 16 ? G.group : 16;  // columns a row
-    const int h0 = g * G.group + slice * 16;
     const int sub = col / heads;                    // row of the tile
     const bool live = sub < per_tile && slice * 16 + col % heads < G.group;
-    const int head = h0 + (live ? col % heads : 0);
-    const float sl2 = G.scale * kLog2e;
-    const int gpb = G.block >> 4;
-    const unsigned tile_mask = (1u << per_tile) - 1;
+    const int head = g * G.group + slice * 16 + (live ? col % heads : 0);
+    const float sl2 = fmaxf(fabsf(G.scale) * kLog2e, 1e-37f);  // a negative scale's sign goes to q; 0 x -inf is no score
 
     for (int a = t0; a < t1;) {
         Seq sq;
@@ -199,22 +198,26 @@ __global__ void __launch_bounds__(256, NT > 1 ? 2 : 1)
             continue;
         }
         const int z = sq.q_base + sq.q_len < t1 ? (int)(sq.q_base + sq.q_len) : t1;
-        // the cursors' rows; a column's row is lane x * per_tile + sub
+        // lane i's row for the walk; a column's row is number (wave * NT + x) * per_tile + sub
         const int t_mine = t0 + lane;
-        const bool row_live = lane < per_wave && t_mine >= a && t_mine < z;
-        const int limit = row_live ? visible_keys(G, sq, (int)(t_mine - sq.q_base)) : 0;
+        const int limit = t_mine >= a && t_mine < z ? visible_keys(G, sq, (int)(t_mine - sq.q_base)) : 0;
         Frag<T> qf[NT][KS];
-        int lim[NT];
+        int lim[NT], num[NT];
 #pragma unroll
         for (int x = 0; x < NT; x++) {
-            const int tx = t0 + x * per_tile + sub;
-            const bool on = live && tx >= a && tx < z;
-            lim[x] = __shfl(limit, x * per_tile + (sub < per_tile ? sub : 0));
+            num[x] = (wave * NT + x) * per_tile + (sub < per_tile ? sub : 0);
+            const bool on = live && t0 + num[x] >= a && t0 + num[x] < z;
+            lim[x] = __shfl(limit, num[x]);
             if (!on) lim[x] = 0;
-            row_frags<T, KS, FULL>(qf[x], q + (long long)(on ? tx : a) * G.q_row + (long long)head * G.q_head, quad, D, on);
+            row_frags<T, KS, false>(qf[x], q + (long long)(on ? t0 + num[x] : a) * G.q_row + (long long)head * G.q_head, quad, D, on);
+            if (G.scale < 0) {
+#pragma unroll
+                for (int w = 0; w < KS; w++) frag_negate(qf[x][w]);
+            }
         }
-        const unsigned every = (z - a < 32 ? (1u << (z - a)) - 1 : ~0u) << (a - t0);
-        unsigned todo = every, now = every;
+        const int count = z - a;
+        const unsigned long long every = (count < 64 ? (1ULL << count) - 1 : ~0ULL) << (a - t0);
+        unsigned long long todo = every, now = every;
         while (todo) {
             f32x4 o[NT][E];
             float m[NT], l[NT];
@@ -225,127 +228,111 @@ __global__ void __launch_bounds__(256, NT > 1 ? 2 : 1)
 #pragma unroll
                 for (int j = 0; j < E; j++) o[x][j] = f32x4{0, 0, 0, 0};
             }
-            Cursors cur = cursor_open(idx + ((long long)(row_live ? t_mine : a) * G.kv_heads + g) * G.width, G.width,
-                                      (limit + G.block - 1) / G.block, row_live && ((now >> (lane & 31)) & 1));
-            unsigned who = 0;
-            int b = cursors_next(cur, who), part = 0;
-            while (b != kNone) {
-                // NG groups of sixteen keys
-                long long k_off[NG], v_off[NG];
-                int rows[NG], from[NG];
-                unsigned whos[NG], any = 0;
-                bool whole = true;
-#pragma unroll
-                for (int y = 0; y < NG; y++) {
-                    if (part == gpb) {
-                        part = 0;
-                        b = cursors_next(cur, who);
+            const int blocks = (read_lane(limit, 63 - __builtin_clzll(now)) + G.block - 1) / G.block;
+            for (int b0 = 0; b0 < blocks; b0 += kRange) {
+                union_build(un, G, idx, g, t0, now, limit, b0, blocks - b0 < kRange ? blocks - b0 : kRange, wave);
+                const int steps = walk_steps<NG, WIDE>(G, un);
+                if (steps == 0) continue;
+                Step<NG, WIDE> st;
+                walk_step<NG, WIDE>(st, G, sq, g, un, b0, limit, 0);
+                tile_load<T, DP, NG, WIDE>(kt[0], k, st.k_off, st, G.k_row, D);
+                tile_load<T, DP, NG, WIDE>(vt[0], v, st.v_off, st, G.v_row, D);
+                __syncthreads();
+                for (int step = 0; step < steps; step++) {
+                    const int buf = step & 1;
+                    const bool more = step + 1 < steps;
+                    Step<NG, WIDE> next = st;
+                    if (more) {
+                        walk_step<NG, WIDE>(next, G, sq, g, un, b0, limit, step + 1);
+                        tile_load<T, DP, NG, WIDE>(kt[buf ^ 1], k, next.k_off, next, G.k_row, D);
+                        tile_load<T, DP, NG, WIDE>(vt[buf ^ 1], v, next.v_off, next, G.v_row, D);
                     }
-                    k_off[y] = (long long)g * G.k_head;
-                    v_off[y] = (long long)g * G.v_head;
-                    rows[y] = 0;
-                    from[y] = 0;
-                    whos[y] = 0;
-                    if (b != kNone) {
-                        // the last of the listing rows sees the most
-                        const int start = b * G.block + part * 16;
-                        const int left = read_lane(limit, 31 - __builtin_clz(who)) - start;
-                        long long kr, vr;
-                        bool there = left > 0;
-                        if (G.page_size > 0) {
-                            const long long page = page_of_block(G, sq.s, b);
-                            there = there && page >= 0;
-                            const long long in = (long long)(b % G.per_page) * G.block + part * 16;
-                            kr = page * G.k_page + in * G.k_row;
-                            vr = page * G.v_page + in * G.v_row;
+                    const bool use = (st.any >> (wave * NT * per_tile)) & (NT * per_tile < 64 ? (1ULL << (NT * per_tile)) - 1 : ~0ULL);
+                    Frag<T> pf[NT][NG / 2];
+                    if (use) {
+                        f32x4 s[NT][NG];
+#pragma unroll
+                        for (int y = 0; y < NG; y++)
+#pragma unroll
+                            for (int x = 0; x < NT; x++) s[x][y] = f32x4{0, 0, 0, 0};
+                        pipelined<Frag<T>, NG * KS, 4, 2>(
+                            [&](int i) { return tile_frag<T, DP>(kt[buf], 16 * (i / KS) + col, i % KS, quad); },
+                            [&](int i, const Frag<T> &f) {
+#pragma unroll
+                                for (int x = 0; x < NT; x++) s[x][i / KS] = mma(f, qf[x][i % KS], s[x][i / KS]);
+                            });
+#pragma unroll
+                        for (int x = 0; x < NT; x++) {
+                            bool on[NG];
+                            bool all = WIDE;
+#pragma unroll
+                            for (int y = 0; y < NG; y++) on[y] = (st.lists(y) >> num[x]) & 1;
+                            if (WIDE) all = __all(!on[0] || lim[x] - st.from[0] >= 16 * NG);
+                            if (!all) {
+                                // some column does not see every key of a block that it lists
+#pragma unroll
+                                for (int y = 0; y < NG; y++) {
+                                    const int vis = on[y] ? lim[x] - st.first(y) - 4 * quad : 0;
+#pragma unroll
+                                    for (int e = 0; e < 4; e++) s[x][y][e] = e < vis ? s[x][y][e] : -INFINITY;
+                                }
+                            }
+                            float top = -INFINITY;
+#pragma unroll
+                            for (int y = 0; y < NG; y++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) top = fmaxf(top, s[x][y][e]);
+                            top = quads_max(top) * sl2;
+                            if (WIDE && !on[0]) top = -INFINITY;
+                            // the maximum need not be the true one: sums of powers up to 2^8 are as exact
+                            if (__any(top > m[x] + 8.f)) {
+                                const float m_new = fmaxf(m[x], top);
+                                const float alpha = pow2(m[x] - (m_new == -INFINITY ? 0.f : m_new));
+                                l[x] *= alpha;
+#pragma unroll
+                                for (int j = 0; j < E; j++) o[x][j] *= alpha;
+                                m[x] = m_new;
+                            }
+                            // columns that do not list the block: 2^-inf
+                            const float base = (WIDE && !on[0]) ? INFINITY : m[x] == -INFINITY ? 0.f : m[x];
+#pragma unroll
+                            for (int y = 0; y < NG; y++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    s[x][y][e] = pow2(__builtin_fmaf(s[x][y][e], sl2, -base));
+                                    l[x] += s[x][y][e];
+                                }
+#pragma unroll
+                            for (int y = 0; y < NG; y += 2) pf[x][y / 2] = frag_pack<T>(s[x][y], s[x][y + 1]);
+                        }
+                    }
+                    if (use) {
+                        if constexpr (sizeof(T) == 2) {
+                            pipelined<Frag<T>, NG / 2 * E, 4, 2>(
+                                [&](int i) { return Columns<T, DP>(vt[buf], 2 * (i / E), quad, col).frag(i % E); },
+                                [&](int i, const Frag<T> &f) {
+#pragma unroll
+                                    for (int x = 0; x < NT; x++) o[x][i % E] = mma(f, pf[x][i / E], o[x][i % E]);
+                                });
                         } else {
-                            kr = (sq.k_base + start) * G.k_row;
-                            vr = (sq.k_base + start) * G.v_row;
+#pragma unroll
+                            for (int y = 0; y < NG; y += 2) {
+                                const Columns<T, DP> c(vt[buf], y, quad, col);
+#pragma unroll
+                                for (int j = 0; j < E; j++) {
+                                    const Frag<T> f = c.frag(j);
+#pragma unroll
+                                    for (int x = 0; x < NT; x++) o[x][j] = mma(f, pf[x][y / 2], o[x][j]);
+                                }
+                            }
                         }
-                        if (there) {
-                            k_off[y] += kr;
-                            v_off[y] += vr;
-                            rows[y] = left < 16 ? left : 16;
-                            whos[y] = who;
-                            from[y] = start;
-                        }
-                        part++;
                     }
-                    any |= whos[y];
-                    whole = whole && rows[y] == 16;
-                }
-                f32x4 s[NT][NG];
-#pragma unroll
-                for (int y = 0; y < NG; y++) {
-                    const int r = col < rows[y] ? col : 0;
-                    Frag<T> kf[KS];
-                    row_frags<T, KS, FULL>(kf, k + k_off[y] + (long long)r * G.k_row, quad, D, true);
-#pragma unroll
-                    for (int x = 0; x < NT; x++) {
-                        s[x][y] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                        for (int w = 0; w < KS; w++) s[x][y] = mma(kf[w], qf[x][w], s[x][y]);
-                    }
-                }
-                Frag<T> pf[NT][NG / 2];
-#pragma unroll
-                for (int x = 0; x < NT; x++) {
-                    if (NT > 1 && !((any >> (x * per_tile)) & tile_mask)) continue;
-                    // keys of each group that this column's row sees
-                    int vis[NG];
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int y = 0; y < NG; y++) {
-                        vis[y] = ((whos[y] >> (x * per_tile + sub)) & 1) ? lim[x] - from[y] - 4 * quad : 0;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) top = fmaxf(top, e < vis[y] ? s[x][y][e] * sl2 : -INFINITY);
-                    }
-                    top = quads_max(top);
-                    // the maximum need not be the true one: sums of powers up to 2^8 are as exact
-                    if (__any(top > m[x] + 8.f)) {
-                        const float m_new = fmaxf(m[x], top);
-                        const float alpha = pow2(m[x] - (m_new == -INFINITY ? 0.f : m_new));
-                        l[x] *= alpha;
-#pragma unroll
-                        for (int j = 0; j < E; j++) o[x][j] *= alpha;
-                        m[x] = m_new;
-                    }
-                    const float base = m[x] == -INFINITY ? 0.f : m[x];
-#pragma unroll
-                    for (int y = 0; y < NG; y++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            s[x][y][e] = e < vis[y] ? pow2(__builtin_fmaf(s[x][y][e], sl2, -base)) : 0.f;
-                            l[x] += s[x][y][e];
-                        }
-#pragma unroll
-                    for (int y = 0; y < NG; y += 2) pf[x][y / 2] = frag_pack<T>(s[x][y], s[x][y + 1]);
-                }
-#pragma unroll
-                for (int y = 0; y < NG; y += 2) {
-                    Rows<T, E> vr;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const int yy = y + (e >> 2);
-                        const int r = 4 * quad + (e & 3);
-                        const T *p = v + v_off[yy] + (long long)(r < rows[yy] ? r : 0) * G.v_row + col * E;
-                        if constexpr (FULL) rows_load(vr, e, p); else rows_load_part(vr, e, p, D - col * E);
-                        if (!whole && r >= rows[yy]) rows_clear(vr, e);
-                    }
-#pragma unroll
-                    for (int j = 0; j < E; j++) {
-                        const Frag<T> c = rows_column(vr, j);
-#pragma unroll
-                        for (int x = 0; x < NT; x++)
-                            if (NT == 1 || ((any >> (x * per_tile)) & tile_mask)) o[x][j] = mma(c, pf[x][y / 2], o[x][j]);
-                    }
-                }
-                if (part == gpb) {
-                    part = 0;
-                    b = cursors_next(cur, who);
+                    st = next;
+                    __syncthreads();
                 }
             }
-            // A value that one row sees and that is no number reaches the other columns' sums as 0 x NaN: then every row by itself.
+            // A value that is no number reaches the columns that do not see it as 0 x NaN: then every row by itself, whose hidden keys are
+            // zeros in LDS.
             bool bad = false;
 #pragma unroll
             for (int x = 0; x < NT; x++) {
@@ -355,25 +342,16 @@ __global__ void __launch_bounds__(256, NT > 1 ? 2 : 1)
                 for (int j = 0; j < E; j++) t += (o[x][j][0] + o[x][j][1]) + (o[x][j][2] + o[x][j][3]);
                 bad = bad || !(fabsf(t) < INFINITY);
             }
-            if ((now & (now - 1)) && __any(bad)) {
+            if ((now & (now - 1)) && __syncthreads_or(bad)) {
                 now = todo & -todo;
                 continue;
             }
 #pragma unroll
             for (int x = 0; x < NT; x++) {
-                const int tx = t0 + x * per_tile + sub;
-                if (!live || !((now >> (x * per_tile + sub)) & 1)) continue;
-                const float inv = l[x] == 0.f ? 0.f : 1.f / l[x];
-                T *orow = out + ((long long)tx * G.heads + head) * D;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    float w[E];
-#pragma unroll
-                    for (int j = 0; j < E; j++) w[j] = o[x][j][e] * inv;
-                    const int d = (4 * quad + e) * E;
-                    store_columns<T, E>(orow + d, w, D - d);
-                }
-                if (lse && quad == 0) lse[(long long)tx * G.heads + head] = l[x] == 0.f ? -INFINITY : (m[x] + log2f(l[x])) * kLn2;
+                if (!live || !((now >> num[x]) & 1)) continue;
+                const long long th = (long long)(t0 + num[x]) * G.heads + head;
+                store_row<T, DP>(out + th * D, o[x], l[x] == 0.f ? 0.f : 1.f / l[x], quad, D);
+                if (lse && quad == 0) lse[th] = l[x] == 0.f ? -INFINITY : (m[x] + log2f(l[x])) * kLn2;
             }
             todo &= ~now;
             now = todo & -todo;
@@ -388,7 +366,7 @@ static void launch_tiles(const Geometry &G, const void *q, const void *k, const 
     const int slices = (int)ceil_div(G.group, 16);
     const int per_tile = G.group < 16 ? 16 / G.group : 1;
     const dim3 grid((unsigned)(ceil_div(G.q_rows, 4 * NT * per_tile) * slices * G.kv_heads));
-    if (G.head_dim == DP)
+    if (G.block >= 16 * NG)
         hipLaunchKernelGGL((k_attend_tiles<T, DP, NT, NG, true>), grid, dim3(256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx,
                            (T *)out, lse, slices, per_tile);
     else
@@ -407,7 +385,7 @@ static void launch_attend(const Geometry &G, const void *q, const void *k, const
     if (!split && G.q_rows / G.n_seq >= 4) {
         if constexpr (sizeof(T) == 2 && DP <= 128) {
             const int per_tile = G.group < 16 ? 16 / G.group : 1;
-            if (rows * G.kv_heads >= 2 * per_tile * 2048LL) {
+            if (per_tile <= 8 && rows * G.kv_heads >= 2 * per_tile * 2048LL) {
                 launch_tiles<T, DP, 2, NG>(G, q, k, v, idx, out, lse, st);
                 return;
             }

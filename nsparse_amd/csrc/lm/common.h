@@ -76,6 +76,13 @@ template <> __device__ inline Frag<float> frag_zero<float>() { return Frag<float
 template <class T> __device__ inline Frag<T> frag_load(const T *p) { return Frag<T>{*(const u32x4 *)p}; }
 template <> __device__ inline Frag<float> frag_load<float>(const float *p) { return Frag<float>{*(const f32x4 *)p, *(const f32x4 *)(p + 4)}; }
 
+template <class T> __device__ inline void frag_negate(Frag<T> &f) { f.r ^= 0x80008000u; }
+template <> __device__ inline void frag_negate<float>(Frag<float> &f)
+{
+    f.lo = -f.lo;
+    f.hi = -f.hi;
+}
+
 template <class T> __device__ inline float frag_dot(const Frag<T> &a, const Frag<T> &b)
 {
     typedef __attribute__((ext_vector_type(8))) T T8;
@@ -211,19 +218,10 @@ __device__ inline float quads_sum(float x)
     r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-// the least of the first 32 lanes, in a scalar register
-__device__ inline int least_of_32(int x)
+__device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ inline unsigned long long uniform64(unsigned long long v)
 {
-    int o = __builtin_amdgcn_mov_dpp(x, 0xb1, 0xf, 0xf, false);  // neighbours
-    x = o < x ? o : x;
-    o = __builtin_amdgcn_mov_dpp(x, 0x4e, 0xf, 0xf, false);  // pairs
-    x = o < x ? o : x;
-    o = __builtin_amdgcn_mov_dpp(x, 0x141, 0xf, 0xf, false);  // mirrored halves of 16
-    x = o < x ? o : x;
-    o = __builtin_amdgcn_mov_dpp(x, 0x140, 0xf, 0xf, false);  // mirrored 16
-    x = o < x ? o : x;
-    const int a = read_lane(x, 0), b = read_lane(x, 16);
-    return a < b ? a : b;
+    return ((unsigned long long)(unsigned)uniform((int)(v >> 32)) << 32) | (unsigned)uniform((int)v);
 }
 // 2^x in one instruction; what is below 2^-126 becomes 0, which no sum next to a 1 can tell
 __device__ inline float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
