@@ -89,12 +89,13 @@ struct Union {
 __device__ inline void union_build(Union &u, const Geometry &G, const int *idx, int g, int t0, unsigned long long now, int limit, int b0, int nb,
                                    int wave)
 {
+    const int lane = opaque(lane_id());
     __syncthreads();
-    for (int x = threadIdx.x; x < nb; x += 256) u.who[x] = 0;
+    for (int x = wave * 64 + lane; x < nb; x += 256) u.who[x] = 0;
     __syncthreads();
     if (G.width <= 16) {
         // four rows at a time, sixteen lanes each; all of them are on their way before the first is looked at
-        const int sub = lane_id() >> 4, j = lane_id() & 15;
+        const int sub = lane >> 4, j = lane & 15;
         int e[4];
 #pragma unroll
         for (int p = 0; p < 4; p++) {
@@ -115,7 +116,7 @@ __device__ inline void union_build(Union &u, const Geometry &G, const int *idx, 
             o = __builtin_amdgcn_update_dpp(-1, top, 0x118, 0xf, 0xf, false);
             top = o > top ? o : top;
             const int before = __builtin_amdgcn_update_dpp(-1, top, 0x111, 0xf, 0xf, false);
-            const int lim = __shfl(limit, n), b = e[p];
+            const int lim = pull(limit, n), b = e[p];
             if (b > before && (long long)b * G.block < lim && b >= b0 && b < b0 + nb) atomicOr((unsigned *)&u.who[b - b0] + (n >> 5), 1u << (n & 31));
         }
     } else {
@@ -127,7 +128,7 @@ __device__ inline void union_build(Union &u, const Geometry &G, const int *idx, 
             for (int at = 0; at < G.width; at += 64) {
                 int b;
                 const int c = pattern_chunk(row, at, G.width, (lim + G.block - 1) / G.block, seen, b);
-                if (lane_id() < c && b >= b0 && b < b0 + nb) atomicOr((unsigned *)&u.who[b - b0] + (n >> 5), 1u << (n & 31));
+                if (lane < c && b >= b0 && b < b0 + nb) atomicOr((unsigned *)&u.who[b - b0] + (n >> 5), 1u << (n & 31));
             }
         }
     }
@@ -135,15 +136,32 @@ __device__ inline void union_build(Union &u, const Geometry &G, const int *idx, 
     if (wave == 0) {
         int n = 0;
         for (int x = 0; x < nb; x += 64) {
-            const bool in = x + lane_id() < nb && u.who[x + lane_id()] != 0;
+            const bool in = x + lane < nb && u.who[x + lane] != 0;
             const unsigned long long m = __ballot(in);
-            if (in) u.list[n + __popcll(m & ((1ULL << lane_id()) - 1))] = (unsigned short)(x + lane_id());
+            if (in) u.list[n + __popcll(m & ((1ULL << lane) - 1))] = (unsigned short)(x + lane);
             n += __popcll(m);
         }
-        if (lane_id() == 0) u.n = n;
+        if (lane == 0) u.n = n;
     }
     __syncthreads();
 }
+
+// What a column of a wavefront's products stands for: the tile's row `sub` and a query head.  Asked for where it is needed.
+struct Column {
+    int col, quad, sub, head;
+    bool live;
+    __device__ inline Column(const Geometry &G, int g, int slice, int per_tile)
+    {
+        const int lane = opaque(lane_id());
+        col = lane & 15;
+        quad = lane >> 4;
+        const int heads = G.group < 16 ? G.group : 16;  // columns a row
+        sub = col / heads;
+        live = sub < per_tile && slice * 16 + col % heads < G.group;
+        head = g * G.group + slice * 16 + (live ? col % heads : 0);
+        if (sub >= per_tile) sub = 0;
+    }
+};
 
 // NG groups of sixteen keys of a walk.  WIDE: a block has at least as many, they are neighbours; else up to NG blocks.
 template <int NG, bool WIDE> struct Step {
@@ -284,7 +302,8 @@ __device__ inline void tile_load(u32x4 *t, const T *p, const long long (&off)[WI
     constexpr int kRows = 256 / kPieces;  // rows a pass
     constexpr int kPasses = NG * 16 / kRows;
     static_assert(kRows <= 16 || kRows % 16 == 0, "a pass covers whole groups or a part of one");
-    const int at = (int)threadIdx.x % kPieces, r0 = (int)threadIdx.x / kPieces;
+    const int tid = opaque((int)threadIdx.x);
+    const int at = tid % kPieces, r0 = tid / kPieces;
     bool whole = head_dim == DP;
 #pragma unroll
     for (int y = 0; y < NG; y++) whole = whole && s.rows(y) >= 16;
@@ -310,12 +329,12 @@ __device__ inline void tile_load(u32x4 *t, const T *p, const long long (&off)[WI
         }
         if (whole) {
             // lane i's 16 bytes land at the wavefront's base + 16 i
-            u32x4 *base = t + i * 256 + uniform((int)(threadIdx.x & ~63u));
+            u32x4 *base = t + i * 256 + uniform(tid & ~63);
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(p + o), (__attribute__((address_space(3))) void *)base, 16, 0, 0);
         } else {
             u32x4 x = u32x4{0, 0, 0, 0};
             if ((r & 15) < n && c < head_dim) x = *(const u32x4 *)(p + o);
-            t[i * 256 + threadIdx.x] = x;
+            t[i * 256 + tid] = x;
         }
     }
 }

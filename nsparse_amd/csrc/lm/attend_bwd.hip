@@ -14,101 +14,200 @@ namespace nsp {
 namespace lm {
 
 // ---- dq (and delta) ----------------------------------------------------------------------------------------------------
-template <class T, int DP, int NG, bool FULL>
-__global__ void __launch_bounds__(256)
+// As the forward for prompts (attend_fwd.hip): the workgroup's rows are the columns of its products, the union of their blocks goes
+// through LDS.  S^T = K Q^T and dP^T = V dO^T read K and V by rows, dQ^T = K^T dS^T reads K transposed.
+// delta comes from the output as the forward rounded it.  That rounding matters where few keys share the weight, so workgroups with
+// at most kExact keys in their union walk twice and take delta = sum p (dout . v) from the first walk.  In single precision the
+// probabilities are divided by their sum, which takes the rounding of the log-sum-exp out of them.
+constexpr int kExact = 256;
+struct RowInfo {  // of a query row and head, for dk and dv
+    float lse2, delta, inv;
+    float pad;
+};
+template <class T, int DP, int NT, int NG, bool WIDE>
+__global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
     k_attend_dq(const Geometry G, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ idx,
                 const T *__restrict__ out, const float *__restrict__ lse, const T *__restrict__ dout, T *__restrict__ dq,
-                float *__restrict__ delta, int slices)
+                RowInfo *__restrict__ info, int slices, int per_tile)
 {
-    constexpr int KS = DP / 32, E = DP / 16;
-    const int lane = lane_id(), col = lane & 15, quad = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    constexpr int KS = DP / 32, E = DP / 16, kTile = NG * 16 * Tile<T, DP>::kPieces;
+    __shared__ u32x4 kt[2][kTile], vt[2][kTile];
+    __shared__ Union un;
+    const int wave = uniform((int)(threadIdx.x >> 6));
     const int g = (int)(blockIdx.x % G.kv_heads);
     const int rest = (int)(blockIdx.x / G.kv_heads);
     const int slice = rest % slices;
-    const int t = (rest / slices) * 4 + wave;
-    if (t >= G.q_rows) return;
-    Seq sq;
-    const int i = seq_of_query(G, t, sq);
-    if (i < 0) return;
-    const int limit = visible_keys(G, sq, i);
+    const int per_wave = NT * per_tile;  // rows a wavefront
+    const int t0 = (rest / slices) * 4 * per_wave;
+    const int t1 = t0 + 4 * per_wave < G.q_rows ? t0 + 4 * per_wave : G.q_rows;
     const int D = G.head_dim;
-    const int h0 = g * G.group + slice * 16;
-    const int nh = G.group - slice * 16 < 16 ? G.group - slice * 16 : 16;
-    const bool live = col < nh;
-    const long long orow = ((long long)t * G.heads + h0 + col) * D;
-
-    Frag<T> qf[KS], gf[KS];
-    float dl = 0.f;
-    row_frags<T, KS, FULL>(gf, dout + orow, quad, D, live);
-    row_frags<T, KS, FULL>(qf, out + orow, quad, D, live);
-#pragma unroll
-    for (int z = 0; z < KS; z++) dl += frag_dot(gf[z], qf[z]);
-    dl = quads_sum(dl);
-    if (quad == 0 && live) delta[(long long)t * G.heads + h0 + col] = dl;
-    row_frags<T, KS, FULL>(qf, q + (long long)t * G.q_row + (long long)(h0 + col) * G.q_head, quad, D, live);
-    const float lse2 = live ? lse[(long long)t * G.heads + h0 + col] * kLog2e : INFINITY;
     const float sl2 = G.scale * kLog2e;
-    f32x4 o[E];
+
+    for (int a = t0; a < t1;) {
+        Seq sq;
+        const int i0 = seq_of_query(G, a, sq);
+        if (i0 < 0) {
+            a++;
+            continue;
+        }
+        const int z = sq.q_base + sq.q_len < t1 ? (int)(sq.q_base + sq.q_len) : t1;
+        const Column c0(G, g, slice, per_tile);
+        const int col = c0.col, quad = c0.quad;
+        // lane i's row for the walk; a column's row is number (wave * NT + x) * per_tile + Column::sub
+        const int t_mine = t0 + opaque(lane_id());
+        const int limit = t_mine >= a && t_mine < z ? visible_keys(G, sq, (int)(t_mine - sq.q_base)) : 0;
+        Frag<T> qf[NT][KS], gf[NT][KS];
+        int lim[NT], num[NT];
+        float lse2[NT], rounded[NT];
 #pragma unroll
-    for (int j = 0; j < E; j++) o[j] = f32x4{0, 0, 0, 0};
-    const int shift = 27 - __builtin_clz(G.block);
-    const int *row = idx + ((long long)t * G.kv_heads + g) * G.width;
-    int seen = -1;
-    for (int at = 0; at < G.width && limit > 0; at += 64) {
-        const Chunk c = chunk_of_row(G, sq, g, row, at, limit, seen);
-        const int total = c.n << shift;
-        for (int u = 0; u < total; u += NG) {
-            Group16 x[NG];
-            bool whole = true;
+        for (int x = 0; x < NT; x++) {
+            num[x] = (wave * NT + x) * per_tile + c0.sub;
+            const bool on = c0.live && t0 + num[x] >= a && t0 + num[x] < z;
+            lim[x] = pull(limit, num[x]);
+            if (!on) lim[x] = 0;
+            const int t = on ? t0 + num[x] : a;
+            const long long th = (long long)t * G.heads + c0.head;
+            row_frags<T, KS, false>(gf[x], dout + th * D, quad, D, on);
+            row_frags<T, KS, false>(qf[x], out + th * D, quad, D, on);
+            rounded[x] = 0.f;
 #pragma unroll
-            for (int y = 0; y < NG; y++) {
-                x[y] = group_of_chunk(G, c, u + y, shift, g);
-                whole = whole && x[y].rows == 16;
+            for (int w = 0; w < KS; w++) rounded[x] += frag_dot(gf[x][w], qf[x][w]);
+            rounded[x] = quads_sum(rounded[x]);
+            row_frags<T, KS, false>(qf[x], q + (long long)t * G.q_row + (long long)c0.head * G.q_head, quad, D, on);
+            lse2[x] = on ? lse[th] * kLog2e : INFINITY;
+        }
+        const int count = z - a;
+        const unsigned long long every = (count < 64 ? (1ULL << count) - 1 : ~0ULL) << (a - t0);
+        unsigned long long todo = every, now = every;
+        while (todo) {
+            f32x4 o[NT][E];
+            float total[NT], with_dp[NT], delta[NT];
+#pragma unroll
+            for (int x = 0; x < NT; x++) {
+                total[x] = with_dp[x] = 0.f;
+                delta[x] = rounded[x];
+#pragma unroll
+                for (int j = 0; j < E; j++) o[x][j] = f32x4{0, 0, 0, 0};
             }
-            f32x4 s[NG];
+            const int blocks = (read_lane(limit, 63 - __builtin_clzll(now)) + G.block - 1) / G.block;
+            for (int b0 = 0; b0 < blocks; b0 += kRange) {
+                union_build(un, G, idx, g, t0, now, limit, b0, blocks - b0 < kRange ? blocks - b0 : kRange, wave);
+                const int steps = walk_steps<NG, WIDE>(G, un);
+                if (steps == 0) continue;
+                const bool exact = sizeof(T) == 2 && blocks <= kRange && steps * NG * 16 <= kExact;
+                for (int pass = exact ? 0 : 1; pass < 2; pass++) {
+                    Step<NG, WIDE> st;
+                    walk_step<NG, WIDE>(st, G, sq, g, un, b0, limit, 0);
+                    tile_load<T, DP, NG, WIDE>(kt[0], k, st.k_off, st, G.k_row, D);
+                    tile_load<T, DP, NG, WIDE>(vt[0], v, st.v_off, st, G.v_row, D);
+                    __syncthreads();
+                    for (int step = 0; step < steps; step++) {
+                        const int buf = step & 1;
+                        Step<NG, WIDE> next = st;
+                        if (step + 1 < steps) {
+                            walk_step<NG, WIDE>(next, G, sq, g, un, b0, limit, step + 1);
+                            tile_load<T, DP, NG, WIDE>(kt[buf ^ 1], k, next.k_off, next, G.k_row, D);
+                            tile_load<T, DP, NG, WIDE>(vt[buf ^ 1], v, next.v_off, next, G.v_row, D);
+                        }
+                        const bool use = (st.any >> (wave * NT * per_tile)) & (NT * per_tile < 64 ? (1ULL << (NT * per_tile)) - 1 : ~0ULL);
+                        if (use) {
 #pragma unroll
-            for (int y = 0; y < NG; y++) {
-                const int r = col < x[y].rows ? col : 0;
-                Frag<T> f[KS];
-                f32x4 dp = f32x4{0, 0, 0, 0};
-                s[y] = f32x4{0, 0, 0, 0};
-                row_frags<T, KS, FULL>(f, k + x[y].k_off + (long long)r * G.k_row, quad, D, true);
+                            for (int y2 = 0; y2 < NG; y2 += 2) {
+                                Frag<T> pf[NT];
+                                f32x4 s[NT][2], d[NT][2];
 #pragma unroll
-                for (int z = 0; z < KS; z++) s[y] = mma(f[z], qf[z], s[y]);
-                row_frags<T, KS, FULL>(f, v + x[y].v_off + (long long)r * G.v_row, quad, D, true);
+                                for (int x = 0; x < NT; x++) s[x][0] = s[x][1] = d[x][0] = d[x][1] = f32x4{0, 0, 0, 0};
+                                pipelined<Frag<T>, 4 * KS, 4, 2>(
+                                    [&](int i) {
+                                        const int r = 16 * (y2 + (i / KS & 1)) + col;
+                                        return tile_frag<T, DP>(i < 2 * KS ? kt[buf] : vt[buf], r, i % KS, quad);
+                                    },
+                                    [&](int i, const Frag<T> &f) {
+                                        const int y = i / KS & 1;
 #pragma unroll
-                for (int z = 0; z < KS; z++) dp = mma(f[z], gf[z], dp);
+                                        for (int x = 0; x < NT; x++) {
+                                            if (i < 2 * KS) s[x][y] = mma(f, qf[x][i % KS], s[x][y]);
+                                            else d[x][y] = mma(f, gf[x][i % KS], d[x][y]);
+                                        }
+                                    });
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    s[y][e] = (4 * quad + e < x[y].rows && live) ? exp2f(s[y][e] * sl2 - lse2) * (dp[e] - dl) * G.scale : 0.f;
-            }
+                                for (int x = 0; x < NT; x++) {
 #pragma unroll
-            for (int y = 0; y < NG; y += 2) {
-                Rows<T, E> kr;
+                                    for (int y = 0; y < 2; y++) {
+                                        const bool on = (st.lists(y2 + y) >> num[x]) & 1;
+                                        const int vis = on ? lim[x] - st.first(y2 + y) - 4 * quad : 0;
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const Group16 &gx = x[y + (e >> 2)];
-                    const int r = 4 * quad + (e & 3);
-                    const T *p = k + gx.k_off + (long long)(r < gx.rows ? r : 0) * G.k_row + col * E;
-                    if constexpr (FULL) rows_load(kr, e, p); else rows_load_part(kr, e, p, D - col * E);
-                    if (!whole && r >= gx.rows) rows_clear(kr, e);
+                                        for (int e = 0; e < 4; e++) {
+                                            const float p = e < vis ? pow2(__builtin_fmaf(s[x][y][e], sl2, -lse2[x])) : 0.f;
+                                            if (pass == 0) with_dp[x] += p * d[x][y][e];
+                                            if (pass == 0 || sizeof(T) == 4) total[x] += p;
+                                            s[x][y][e] = p * (d[x][y][e] - delta[x]) * G.scale;
+                                        }
+                                    }
+                                    pf[x] = frag_pack<T>(s[x][0], s[x][1]);
+                                }
+                                if (pass == 0) continue;
+                                if constexpr (sizeof(T) == 2) {
+                                    pipelined<Frag<T>, E, 4, 2>([&](int i) { return Columns<T, DP>(kt[buf], y2, quad, col).frag(i); },
+                                                                [&](int i, const Frag<T> &f) {
+#pragma unroll
+                                                                    for (int x = 0; x < NT; x++) o[x][i] = mma(f, pf[x], o[x][i]);
+                                                                });
+                                } else {
+                                    const Columns<T, DP> c(kt[buf], y2, quad, col);
+#pragma unroll
+                                    for (int j = 0; j < E; j++) {
+                                        const Frag<T> f = c.frag(j);
+#pragma unroll
+                                        for (int x = 0; x < NT; x++) o[x][j] = mma(f, pf[x], o[x][j]);
+                                    }
+                                }
+                            }
+                        }
+                        st = next;
+                        __syncthreads();
+                    }
+                    if (pass == 0) {
+#pragma unroll
+                        for (int x = 0; x < NT; x++) {
+                            const float w = quads_sum(with_dp[x]), l = quads_sum(total[x]);
+                            delta[x] = l > 0.f ? w / l : 0.f;
+                            total[x] = 0.f;
+                        }
+                    }
                 }
-                const Frag<T> sf = frag_pack<T>(s[y], s[y + 1]);
-#pragma unroll
-                for (int j = 0; j < E; j++) o[j] = mma(rows_column(kr, j), sf, o[j]);
             }
-        }
-    }
-    if (live) {
+            // A value that is no number reaches the columns that do not see it as 0 x NaN: then every row by itself.
+            bool bad = false;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            float w[E];
+            for (int x = 0; x < NT; x++) {
+                float t = delta[x];
 #pragma unroll
-            for (int j = 0; j < E; j++) w[j] = o[j][e];
-            const int d = (4 * quad + e) * E;
-            store_columns<T, E>(dq + orow + d, w, D - d);
+                for (int j = 0; j < E; j++) t += (o[x][j][0] + o[x][j][1]) + (o[x][j][2] + o[x][j][3]);
+                bad = bad || !(fabsf(t) < INFINITY);
+            }
+            if ((now & (now - 1)) && __syncthreads_or(bad)) {
+                now = todo & -todo;
+                continue;
+            }
+            const Column c1(G, g, slice, per_tile);
+#pragma unroll
+            for (int x = 0; x < NT; x++) {
+                float inv = 1.f;
+                if (sizeof(T) == 4) {
+                    const float l = quads_sum(total[x]);
+                    inv = l > 0.f ? 1.f / l : 1.f;
+                }
+                const int n = (wave * NT + x) * per_tile + c1.sub;
+                if (!c1.live || !((now >> n) & 1)) continue;
+                const long long th = (long long)(t0 + n) * G.heads + c1.head;
+                store_row<T, DP>(dq + th * D, o[x], inv, c1.quad, D);
+                if (c1.quad == 0) info[th] = RowInfo{lse2[x], delta[x], inv, 0.f};
+            }
+            todo &= ~now;
+            now = todo & -todo;
         }
+        a = z;
     }
 }
 
@@ -171,8 +270,8 @@ __global__ void __launch_bounds__(256)
 constexpr int kListWords = 64;
 template <class T, int DP, bool FULL>
 __global__ void __launch_bounds__(256)
-    k_attend_dkv(const Geometry G, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const float *__restrict__ lse,
-                 const T *__restrict__ dout, const float *__restrict__ delta, const unsigned long long *__restrict__ bits, T *__restrict__ dk,
+    k_attend_dkv(const Geometry G, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
+                 const T *__restrict__ dout, const RowInfo *__restrict__ rinfo, const unsigned long long *__restrict__ bits, T *__restrict__ dk,
                  T *__restrict__ dv, long long mean_rows, int words, int parts)
 {
     constexpr int KS = DP / 32, E = DP / 16;
@@ -180,7 +279,7 @@ __global__ void __launch_bounds__(256)
     __shared__ int listed;
     struct Info {
         long long q_off[32], o_off[32];
-        float lse2[32], delta[32];
+        float lse2[32], delta[32], inv[32];
         int limit[32];
     };
     __shared__ Info infos[4];
@@ -239,8 +338,10 @@ __global__ void __launch_bounds__(256)
                 const long long th = (long long)t * G.heads + h;
                 in.q_off[lane] = (long long)t * G.q_row + (long long)h * G.q_head;
                 in.o_off[lane] = th * D;
-                in.lse2[lane] = lse[th] * kLog2e;
-                in.delta[lane] = delta[th];
+                const RowInfo ri = rinfo[th];
+                in.lse2[lane] = ri.lse2;
+                in.delta[lane] = ri.delta;
+                in.inv[lane] = ri.inv;
                 in.limit[lane] = ok ? visible_keys(G, sq, (int)(t - sq.q_base)) : 0;
             }
             __builtin_amdgcn_wave_barrier();
@@ -262,7 +363,8 @@ __global__ void __launch_bounds__(256)
                 for (int e = 0; e < 4; e++) {
                     const int r = 16 * y + 4 * quad + e;
                     const bool on = mine && key < in.limit[r];
-                    s[y][e] = on ? exp2f(s[y][e] * sl2 - in.lse2[r]) : 0.f;
+                    s[y][e] = on ? pow2(__builtin_fmaf(s[y][e], sl2, -in.lse2[r])) : 0.f;
+                    if (sizeof(T) == 4) s[y][e] *= in.inv[r];
                     ds[y][e] = on ? s[y][e] * (dp[e] - in.delta[r]) * G.scale : 0.f;
                 }
             }
@@ -311,7 +413,7 @@ __global__ void __launch_bounds__(256)
 }
 
 struct BwdSpace {
-    long long mean_rows, delta_bytes, total;
+    long long mean_rows, info_bytes, total;
     int words;
 };
 static BwdSpace bwd_space(const Geometry &G)
@@ -319,8 +421,8 @@ static BwdSpace bwd_space(const Geometry &G)
     BwdSpace s;
     s.mean_rows = G.cu_k ? G.k_rows / G.block + G.n_seq : (long long)G.blocks_each * G.n_seq;
     s.words = (int)ceil_div(G.q_rows, 64);
-    s.delta_bytes = ceil_div((long long)G.q_rows * G.heads * 4, 256) * 256;
-    s.total = s.delta_bytes + 8 * (long long)G.kv_heads * s.mean_rows * s.words;
+    s.info_bytes = ceil_div((long long)G.q_rows * G.heads * (long long)sizeof(RowInfo), 256) * 256;
+    s.total = s.info_bytes + 8 * (long long)G.kv_heads * s.mean_rows * s.words;
     return s;
 }
 
@@ -328,18 +430,27 @@ template <class T, int DP, int NG>
 static void launch_bwd(const Geometry &G, const void *q, const void *k, const void *v, const int *idx, const void *out, const float *lse,
                        const void *dout, void *dq, void *dk, void *dv, char *ws, const BwdSpace &sp, hipStream_t st)
 {
-    float *delta = (float *)ws;
-    unsigned long long *bits = (unsigned long long *)(ws + sp.delta_bytes);
+    RowInfo *info = (RowInfo *)ws;
+    unsigned long long *bits = (unsigned long long *)(ws + sp.info_bytes);
     const int slices = (int)ceil_div(G.group, 16);
     const bool full = G.head_dim == DP;
     if (G.q_rows > 0) {
-        const dim3 grid((unsigned)(ceil_div(G.q_rows, 4) * slices * G.kv_heads));
-        if (full)
-            hipLaunchKernelGGL((k_attend_dq<T, DP, NG, true>), grid, dim3(256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx,
-                               (const T *)out, lse, (const T *)dout, (T *)dq, delta, slices);
-        else
-            hipLaunchKernelGGL((k_attend_dq<T, DP, NG, false>), grid, dim3(256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx,
-                               (const T *)out, lse, (const T *)dout, (T *)dq, delta, slices);
+        const int per_tile = G.group < 16 ? 16 / G.group : 1;
+#define NSP_GO(NT, WIDE)                                                                                                                     \
+    hipLaunchKernelGGL((k_attend_dq<T, DP, NT, NG, WIDE>), dim3((unsigned)(ceil_div(G.q_rows, 4 * NT * per_tile) * slices * G.kv_heads)), \
+                       dim3(256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx, (const T *)out, lse, (const T *)dout, (T *)dq,    \
+                       info, slices, per_tile)
+        bool two = false;
+        if constexpr (sizeof(T) == 2 && DP <= 128) {
+            two = per_tile <= 8 && (long long)G.q_rows * slices * G.kv_heads >= 2 * per_tile * 2048LL;
+            if (two) {
+                if (G.block >= 16 * NG) NSP_GO(2, true); else NSP_GO(2, false);
+            }
+        }
+        if (!two) {
+            if (G.block >= 16 * NG) NSP_GO(1, true); else NSP_GO(1, false);
+        }
+#undef NSP_GO
         if (sp.mean_rows > 0)
             hipLaunchKernelGGL(k_pattern_bits, dim3((unsigned)((long long)sp.words * G.kv_heads)), dim3(256), 0, st, G, idx, bits,
                                sp.mean_rows, sp.words);
@@ -348,11 +459,11 @@ static void launch_bwd(const Geometry &G, const void *q, const void *k, const vo
         const int parts = G.block > 64 ? G.block / 64 : 1;
         const dim3 grid((unsigned)(sp.mean_rows * G.kv_heads * parts)), block(G.block > 64 ? 256 : 4 * G.block);
         if (full)
-            hipLaunchKernelGGL((k_attend_dkv<T, DP, true>), grid, block, 0, st, G, (const T *)q, (const T *)k, (const T *)v, lse,
-                               (const T *)dout, delta, bits, (T *)dk, (T *)dv, sp.mean_rows, sp.words, parts);
+            hipLaunchKernelGGL((k_attend_dkv<T, DP, true>), grid, block, 0, st, G, (const T *)q, (const T *)k, (const T *)v,
+                               (const T *)dout, info, bits, (T *)dk, (T *)dv, sp.mean_rows, sp.words, parts);
         else
-            hipLaunchKernelGGL((k_attend_dkv<T, DP, false>), grid, block, 0, st, G, (const T *)q, (const T *)k, (const T *)v, lse,
-                               (const T *)dout, delta, bits, (T *)dk, (T *)dv, sp.mean_rows, sp.words, parts);
+            hipLaunchKernelGGL((k_attend_dkv<T, DP, false>), grid, block, 0, st, G, (const T *)q, (const T *)k, (const T *)v,
+                               (const T *)dout, info, bits, (T *)dk, (T *)dv, sp.mean_rows, sp.words, parts);
     }
 }
 

@@ -174,7 +174,6 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
     constexpr int KS = DP / 32, E = DP / 16, kTile = NG * 16 * Tile<T, DP>::kPieces;
     __shared__ u32x4 kt[2][kTile], vt[2][kTile];
     __shared__ Union un;
-    const int lane = lane_id(), col = lane & 15, quad = lane >> 4;
     const int wave = uniform((int)(threadIdx.x >> 6));
     // consecutive workgroups go round the key heads: with 8 of them each XCD's cache serves one head's keys
     const int g = (int)(blockIdx.x % G.kv_heads);
@@ -184,10 +183,6 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
     const int t0 = (rest / slices) * 4 * per_wave;
     const int t1 = t0 + 4 * per_wave < G.q_rows ? t0 + 4 * per_wave : G.q_rows;
     const int D = G.head_dim;
-    const int heads = G.group < 16 ? G.group : 16;  // columns a row
-    const int sub = col / heads;                    // row of the tile
-    const bool live = sub < per_tile && slice * 16 + col % heads < G.group;
-    const int head = g * G.group + slice * 16 + (live ? col % heads : 0);
     const float sl2 = fmaxf(fabsf(G.scale) * kLog2e, 1e-37f);  // a negative scale's sign goes to q; 0 x -inf is no score
 
     for (int a = t0; a < t1;) {
@@ -198,18 +193,20 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
             continue;
         }
         const int z = sq.q_base + sq.q_len < t1 ? (int)(sq.q_base + sq.q_len) : t1;
-        // lane i's row for the walk; a column's row is number (wave * NT + x) * per_tile + sub
-        const int t_mine = t0 + lane;
+        const Column c0(G, g, slice, per_tile);
+        const int col = c0.col, quad = c0.quad;
+        // lane i's row for the walk; a column's row is number (wave * NT + x) * per_tile + Column::sub
+        const int t_mine = t0 + opaque(lane_id());
         const int limit = t_mine >= a && t_mine < z ? visible_keys(G, sq, (int)(t_mine - sq.q_base)) : 0;
         Frag<T> qf[NT][KS];
         int lim[NT], num[NT];
 #pragma unroll
         for (int x = 0; x < NT; x++) {
-            num[x] = (wave * NT + x) * per_tile + (sub < per_tile ? sub : 0);
-            const bool on = live && t0 + num[x] >= a && t0 + num[x] < z;
-            lim[x] = __shfl(limit, num[x]);
+            num[x] = (wave * NT + x) * per_tile + c0.sub;
+            const bool on = c0.live && t0 + num[x] >= a && t0 + num[x] < z;
+            lim[x] = pull(limit, num[x]);
             if (!on) lim[x] = 0;
-            row_frags<T, KS, false>(qf[x], q + (long long)(on ? t0 + num[x] : a) * G.q_row + (long long)head * G.q_head, quad, D, on);
+            row_frags<T, KS, false>(qf[x], q + (long long)(on ? t0 + num[x] : a) * G.q_row + (long long)c0.head * G.q_head, quad, D, on);
             if (G.scale < 0) {
 #pragma unroll
                 for (int w = 0; w < KS; w++) frag_negate(qf[x][w]);
@@ -346,12 +343,14 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
                 now = todo & -todo;
                 continue;
             }
+            const Column c1(G, g, slice, per_tile);
 #pragma unroll
             for (int x = 0; x < NT; x++) {
-                if (!live || !((now >> num[x]) & 1)) continue;
-                const long long th = (long long)(t0 + num[x]) * G.heads + head;
-                store_row<T, DP>(out + th * D, o[x], l[x] == 0.f ? 0.f : 1.f / l[x], quad, D);
-                if (lse && quad == 0) lse[th] = l[x] == 0.f ? -INFINITY : (m[x] + log2f(l[x])) * kLn2;
+                const int n = (wave * NT + x) * per_tile + c1.sub;
+                if (!c1.live || !((now >> n) & 1)) continue;
+                const long long th = (long long)(t0 + n) * G.heads + c1.head;
+                store_row<T, DP>(out + th * D, o[x], l[x] == 0.f ? 0.f : 1.f / l[x], c1.quad, D);
+                if (lse && c1.quad == 0) lse[th] = l[x] == 0.f ? -INFINITY : (m[x] + log2f(l[x])) * kLn2;
             }
             todo &= ~now;
             now = todo & -todo;

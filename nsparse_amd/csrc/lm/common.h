@@ -218,6 +218,14 @@ __device__ inline float quads_sum(float x)
     r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+// x, which the compiler cannot know: what depends on it is computed where it is used and not kept in registers over a loop
+__device__ inline int opaque(int x)
+{
+    asm volatile("" : "+v"(x));
+    return x;
+}
+// v of another lane
+__device__ inline int pull(int v, int lane) { return __builtin_amdgcn_ds_bpermute(lane << 2, v); }
 __device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ inline unsigned long long uniform64(unsigned long long v)
 {
@@ -337,15 +345,15 @@ __device__ inline long long page_of_block(const Geometry &G, int s, int b)
 // `seen` carries the greatest entry of the row so far.  Returns how many; `block` is lane i's entry.
 __device__ inline int pattern_chunk(const int *row, int at, int width, int blocks, int &seen, int &block)
 {
-    const int lane = lane_id();
+    const int lane = opaque(lane_id());
     const int e = at + lane < width ? row[at + lane] : -1;
     int top = e;  // greatest entry up to and including this lane
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(top, d);
+        const int o = pull(top, lane - d);
         if (lane >= d) top = top > o ? top : o;
     }
-    int before = __shfl_up(top, 1);
+    int before = pull(top, lane - 1);
     before = lane == 0 ? seen : (before > seen ? before : seen);
     const bool counts = e >= 0 && e < blocks && e > before;
     const unsigned long long mask = __ballot(counts);
