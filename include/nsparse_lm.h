@@ -75,7 +75,7 @@ const char *nsparse_lm_build_info(void);
  */
 typedef struct nsparse_lm_attn {
     int dtype;                  /* of q, k, v, out, dout, dq, dk, dv, means */
-    int heads, kv_heads;        /* heads % kv_heads == 0 */
+    int heads, kv_heads;        /* heads % kv_heads == 0, heads / kv_heads <= 1024 */
     int head_dim;               /* a multiple of 8, at most 256 */
     int block;                  /* keys a block: 16, 32, 64, 128 or 256 */
     int width;                  /* entries of a pattern row: 1 .. 256 */
@@ -83,7 +83,7 @@ typedef struct nsparse_lm_attn {
     int n_seq;
     int page_size;              /* 0, or a multiple of block */
     int first, local;           /* selection: the first and the last eligible blocks always taken; see select_blocks */
-    float scale;                /* of q.k in the softmax */
+    float scale;                /* of q.k in the softmax; finite */
     long long q_rows, k_rows;
     long long table_stride;     /* entries of page_table a sequence */
     const int *cu_q, *cu_k, *q_len, *k_len, *page_table;

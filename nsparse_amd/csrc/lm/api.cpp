@@ -37,8 +37,8 @@ int geometry(const nsparse_lm_attn *a, bool needs_q, bool needs_k, Geometry *g)
     if (!a) return fail(NSPARSE_LM_EARG, "the argument block is NULL");
     if (a->dtype != NSPARSE_LM_F32 && a->dtype != NSPARSE_LM_F16 && a->dtype != NSPARSE_LM_BF16)
         return fail(NSPARSE_LM_ETYPE, "dtype is none of F32, F16, BF16");
-    if (a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->heads > 65536)
-        return fail(NSPARSE_LM_EARG, "heads must be a multiple of kv_heads");
+    if (a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->heads / a->kv_heads > 1024)
+        return fail(NSPARSE_LM_EARG, "heads must be a multiple of kv_heads, at most 1024 times as many");
     if (a->head_dim < 8 || a->head_dim > 256 || a->head_dim % 8) return fail(NSPARSE_LM_EARG, "head_dim must be a multiple of 8 up to 256");
     if (a->block < 16 || a->block > 256 || (a->block & (a->block - 1))) return fail(NSPARSE_LM_EARG, "block must be 16, 32, 64, 128 or 256");
     if (a->width < 1 || a->width > 256) return fail(NSPARSE_LM_EARG, "width must be 1 .. 256");

@@ -212,228 +212,465 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
 }
 
 // ---- the transposed pattern --------------------------------------------------------------------------------------------------
-// bits[(g * mean_rows + mean row) * words + t / 64], bit t % 64: query row t lists the block for head g.  One workgroup
+// bits[(mean row * kv_heads + g) * words + t / 64], bit t % 64: query row t lists the block for head g.  One workgroup
 // makes the words of 64 rows; of each sequence it writes the words of the blocks that its last row there sees.
-constexpr int kBitBlocks = 4096;
 __global__ void __launch_bounds__(256)
-    k_pattern_bits(const Geometry G, const int *__restrict__ idx, unsigned long long *__restrict__ bits, long long mean_rows, int words)
+    k_pattern_bits(const Geometry G, const int *__restrict__ idx, unsigned long long *__restrict__ bits, int words)
 {
-    __shared__ unsigned half[2 * kBitBlocks];
+    __shared__ Union un;
     const int g = (int)(blockIdx.x % G.kv_heads), w = (int)(blockIdx.x / G.kv_heads);
-    const int wave = threadIdx.x >> 6;
+    const int wave = uniform((int)(threadIdx.x >> 6));
     const int t0 = w * 64, t1 = t0 + 64 < G.q_rows ? t0 + 64 : G.q_rows;
-    // the first sequence that reaches into these rows
-    int s = 0;
-    if (G.cu_q) {
-        int hi = G.n_seq;
-        while (hi - s > 1) {
-            const int mid = (s + hi) >> 1;
-            if (G.cu_q[mid] <= t0) s = mid; else hi = mid;
+    for (int a = t0; a < t1;) {
+        Seq sq;
+        const int i0 = seq_of_query(G, a, sq);
+        if (i0 < 0) {
+            a++;
+            continue;
         }
-    } else {
-        s = t0 / G.q_each;
-    }
-    for (; s < G.n_seq; s++) {
-        const Seq sq = seq_at(G, s);
-        if (sq.q_base >= t1) break;
-        const int a = sq.q_base > t0 ? (int)sq.q_base : t0;
         const int z = sq.q_base + sq.q_len < t1 ? (int)(sq.q_base + sq.q_len) : t1;
-        if (z <= a) continue;
-        const int seen_blocks = (visible_keys(G, sq, (int)(z - 1 - sq.q_base)) + G.block - 1) / G.block;
-        for (int b0 = 0; b0 < seen_blocks; b0 += kBitBlocks) {
-            const int nb = seen_blocks - b0 < kBitBlocks ? seen_blocks - b0 : kBitBlocks;
-            for (int x = threadIdx.x; x < 2 * nb; x += 256) half[x] = 0;
-            __syncthreads();
-            for (int t = a + wave; t < z; t += 4) {
-                const int limit = visible_keys(G, sq, (int)(t - sq.q_base));
-                const int *row = idx + ((long long)t * G.kv_heads + g) * G.width;
-                int seen = -1;
-                for (int at = 0; at < G.width; at += 64) {
-                    int b;
-                    const int n = pattern_chunk(row, at, G.width, (limit + G.block - 1) / G.block, seen, b);
-                    if (lane_id() < n && b >= b0 && b < b0 + nb)
-                        atomicOr(&half[2 * (b - b0) + ((t - t0) >> 5)], 1u << ((t - t0) & 31));
-                }
-            }
-            __syncthreads();
-            unsigned long long *p = bits + ((long long)g * mean_rows + mean_base(G, sq) + b0) * words + w;
-            for (int x = threadIdx.x; x < nb; x += 256)
-                p[(long long)x * words] = ((unsigned long long)half[2 * x + 1] << 32) | half[2 * x];
-            __syncthreads();
+        const int t_mine = t0 + lane_id();
+        const int limit = t_mine >= a && t_mine < z ? visible_keys(G, sq, (int)(t_mine - sq.q_base)) : 0;
+        const int count = z - a;
+        const unsigned long long every = (count < 64 ? (1ULL << count) - 1 : ~0ULL) << (a - t0);
+        const int blocks = (read_lane(limit, z - 1 - t0) + G.block - 1) / G.block;
+        for (int b0 = 0; b0 < blocks; b0 += kRange) {
+            const int nb = blocks - b0 < kRange ? blocks - b0 : kRange;
+            union_build(un, G, idx, g, t0, every, limit, b0, nb, wave);
+            unsigned long long *p = bits + ((mean_base(G, sq) + b0) * G.kv_heads + g) * words + w;
+            for (int x = threadIdx.x; x < nb; x += 256) p[(long long)x * G.kv_heads * words] = un.who[x];
         }
+        a = z;
     }
+}
+
+// The words that can name rows which see block b of a sequence.
+__device__ inline void words_of_block(const Geometry &G, const Seq &sq, int b, int &w0, int &w1)
+{
+    long long i0 = G.causal ? (long long)b * G.block - (sq.k_len - sq.q_len) : 0;
+    if (i0 < 0) i0 = 0;
+    w0 = (int)((sq.q_base + i0) >> 6);
+    w1 = sq.q_len > i0 ? (int)((sq.q_base + sq.q_len - 1) >> 6) + 1 : w0;
+}
+
+// A block that many rows list (the first of a sequence, often) is shared out: an item is at most `per_item` of a block's rows.
+struct Item {
+    int gm, chunk, chunks, slot;  // mean row * kv_heads + head; slot of the item's sums where the block has several
+};
+__global__ void __launch_bounds__(256)
+    k_count_chunks(const Geometry G, const unsigned long long *__restrict__ bits, int *__restrict__ chunks, long long gms, int words, int per_item)
+{
+    const long long gm = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (gm >= gms) return;
+    Seq sq;
+    int b, n = 0, w0, w1;
+    if (!block_of_mean_row(G, gm / G.kv_heads, sq, b)) {
+        if (lane_id() == 0) chunks[gm] = 0;
+        return;
+    }
+    words_of_block(G, sq, b, w0, w1);
+    for (int w = w0 + lane_id(); w < w1; w += 64) n += __popcll(bits[gm * words + w]);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
+    if (lane_id() == 0) chunks[gm] = n <= per_item ? 1 : (n + per_item - 1) / per_item;
+}
+__global__ void __launch_bounds__(1024) k_plan_items(const int *__restrict__ chunks, long long gms, Item *__restrict__ items, int *__restrict__ n_items)
+{
+    __shared__ int sums[2][16];
+    const int lane = lane_id(), wave = (int)(threadIdx.x >> 6);
+    int base = 0, slots = 0;
+    for (long long g0 = 0; g0 < gms; g0 += 1024) {
+        const long long gm = g0 + threadIdx.x;
+        const int n = gm < gms ? chunks[gm] : 0, m = n > 1 ? n : 0;
+        int a = n, c = m;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int x = __shfl_up(a, d), y = __shfl_up(c, d);
+            if (lane >= d) {
+                a += x;
+                c += y;
+            }
+        }
+        if (lane == 63) {
+            sums[0][wave] = a;
+            sums[1][wave] = c;
+        }
+        __syncthreads();
+        int at = base + a - n, slot = slots + c - m;
+        for (int w = 0; w < 16; w++) {
+            if (w < wave) {
+                at += sums[0][w];
+                slot += sums[1][w];
+            }
+            base += sums[0][w];
+            slots += sums[1][w];
+        }
+        for (int i = 0; i < n; i++) items[at + i] = Item{(int)gm, i, n, slot + i};
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *n_items = base;
 }
 
 // ---- dk, dv -------------------------------------------------------------------------------------------------------------------
-// One workgroup per (key head, block, 64 of its keys); wavefront x owns sixteen of the keys, as the columns of its products.  The rows
-// are the (query, head) pairs that list the block, 32 at a time.
-constexpr int kListWords = 64;
-template <class T, int DP, bool FULL>
-__global__ void __launch_bounds__(256)
-    k_attend_dkv(const Geometry G, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
-                 const T *__restrict__ dout, const RowInfo *__restrict__ rinfo, const unsigned long long *__restrict__ bits, T *__restrict__ dk,
-                 T *__restrict__ dv, long long mean_rows, int words, int parts)
-{
-    constexpr int KS = DP / 32, E = DP / 16;
-    __shared__ int list[kListWords * 64];
-    __shared__ int listed;
-    struct Info {
-        long long q_off[32], o_off[32];
-        float lse2[32], delta[32], inv[32];
-        int limit[32];
-    };
-    __shared__ Info infos[4];
-    const int lane = lane_id(), col = lane & 15, quad = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int g = (int)(blockIdx.x % G.kv_heads);
-    const long long rest = blockIdx.x / G.kv_heads;
-    const long long mrow = rest / parts;
-    Seq sq;
-    int b;
-    if (!block_of_mean_row(G, mrow, sq, b)) return;
-    const int D = G.head_dim;
-    const int key = b * G.block + (int)(rest % parts) * 64 + wave * 16 + col;  // inside the sequence
-    const bool mine = key < sq.k_len;
-    const long long krow = sq.k_base + (mine ? key : b * G.block);
-    Frag<T> kf[KS], vf[KS];
-    row_frags<T, KS, FULL>(kf, k + krow * G.k_row + (long long)g * G.k_head, quad, D, mine);
-    row_frags<T, KS, FULL>(vf, v + krow * G.v_row + (long long)g * G.v_head, quad, D, mine);
-    f32x4 ak[E], av[E];
-#pragma unroll
-    for (int j = 0; j < E; j++) ak[j] = av[j] = f32x4{0, 0, 0, 0};
-    const float sl2 = G.scale * kLog2e;
-    Info &in = infos[wave];
-    const unsigned long long *mybits = bits + ((long long)g * mean_rows + mrow) * words;
-    // the rows that can see the block's first key
-    int i0 = G.causal ? b * G.block - (sq.k_len - sq.q_len) : 0;
-    if (i0 < 0) i0 = 0;
-    const int w0 = (int)((sq.q_base + i0) >> 6), w1 = sq.q_len > i0 ? (int)((sq.q_base + sq.q_len - 1) >> 6) + 1 : w0;
-    for (int wb = w0; wb < w1; wb += kListWords) {
-        __syncthreads();
-        if (wave == 0) {
-            unsigned long long m = wb + lane < w1 ? mybits[wb + lane] : 0;
-            int at = __popcll(m);
-            int sum = at;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const int o = __shfl_up(sum, d);
-                if (lane >= d) sum += o;
-            }
-            at = sum - at;
-            if (lane == 63) listed = sum;
-            const int t0 = (wb + lane) * 64;
-            while (m) {
-                list[at++] = t0 + __builtin_ctzll(m);
-                m &= m - 1;
-            }
+// An item's workgroup owns up to 64 keys of the block: KEYS wavefronts side by side with KW x 16 keys each, as the columns of their
+// products, and ROWS of them one behind the other, each with its own 32 of the (query, head) pairs that list the block.
+// The pairs' rows of q and dout go through LDS (by rows for S = Q K^T and dP = dO V^T, transposed for dK^T = Q^T dS and
+// dV^T = dO^T P), fetched while the 32 before are computed.  Bound by what LDS delivers: KW = 2 halves the reads a product.
+constexpr int kListed = 1024;
+template <class T, int DP, int KW, int KEYS, int ROWS> struct Dkv {
+    static constexpr int KS = DP / 32, E = DP / 16, kThreads = 64 * KEYS * ROWS, kStep = 32 * ROWS;
+    static constexpr int kPieces = Tile<T, DP>::kPieces, kTile = kStep * kPieces;
+    static constexpr int kDump = KW * 2 * E * 4;  // sums a lane
+    static constexpr int kWaves = DP * sizeof(T) <= 256 && kTile <= 1024 ? 2 : 1;  // a SIMD: what the sums and the tiles leave room for
+    struct Sums {
+        f32x4 k[KW][E], v[KW][E];
+        __device__ inline float &at(int i)
+        {
+            f32x4 &x = i / 4 < KW * E ? k[i / 4 / E][i / 4 % E] : v[(i / 4 - KW * E) / E][i / 4 % E];
+            return ((float *)&x)[i & 3];
         }
-        __syncthreads();
-        const long long rows = (long long)listed * G.group;
-        for (long long r0 = 0; r0 < rows; r0 += 32) {
-            __builtin_amdgcn_wave_barrier();
-            if (lane < 32) {
-                const long long r = r0 + lane;
-                const bool ok = r < rows;
-                const int t = list[ok ? r / G.group : 0], h = g * G.group + (ok ? (int)(r % G.group) : 0);
-                const long long th = (long long)t * G.heads + h;
-                in.q_off[lane] = (long long)t * G.q_row + (long long)h * G.q_head;
-                in.o_off[lane] = th * D;
-                const RowInfo ri = rinfo[th];
-                in.lse2[lane] = ri.lse2;
-                in.delta[lane] = ri.delta;
-                in.inv[lane] = ri.inv;
-                in.limit[lane] = ok ? visible_keys(G, sq, (int)(t - sq.q_base)) : 0;
-            }
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            const bool whole = r0 + 32 <= rows;
-            f32x4 s[2], ds[2];
+    };
+    static __device__ inline void store(const Geometry &G, Sums &a, const Seq &sq, int b, int g, int part, int kw, T *dk, T *dv)
+    {
+        const int lane = opaque(lane_id()), col = lane & 15, quad = lane >> 4;
 #pragma unroll
-            for (int y = 0; y < 2; y++) {
-                Frag<T> f[KS];
-                f32x4 dp = f32x4{0, 0, 0, 0};
-                s[y] = f32x4{0, 0, 0, 0};
-                row_frags<T, KS, FULL>(f, q + in.q_off[16 * y + col], quad, D, true);
-#pragma unroll
-                for (int z = 0; z < KS; z++) s[y] = mma(f[z], kf[z], s[y]);
-                row_frags<T, KS, FULL>(f, dout + in.o_off[16 * y + col], quad, D, true);
-#pragma unroll
-                for (int z = 0; z < KS; z++) dp = mma(f[z], vf[z], dp);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int r = 16 * y + 4 * quad + e;
-                    const bool on = mine && key < in.limit[r];
-                    s[y][e] = on ? pow2(__builtin_fmaf(s[y][e], sl2, -in.lse2[r])) : 0.f;
-                    if (sizeof(T) == 4) s[y][e] *= in.inv[r];
-                    ds[y][e] = on ? s[y][e] * (dp[e] - in.delta[r]) * G.scale : 0.f;
-                }
-            }
-            {
-                Rows<T, E> x;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int r = (e < 4 ? 0 : 16) + 4 * quad + (e & 3);
-                    const T *p = dout + in.o_off[r] + col * E;
-                    if constexpr (FULL) rows_load(x, e, p); else rows_load_part(x, e, p, D - col * E);
-                    if (!whole && r0 + r >= rows) rows_clear(x, e);
-                }
-                const Frag<T> pf = frag_pack<T>(s[0], s[1]);
-#pragma unroll
-                for (int j = 0; j < E; j++) av[j] = mma(rows_column(x, j), pf, av[j]);
-            }
-            {
-                Rows<T, E> x;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int r = (e < 4 ? 0 : 16) + 4 * quad + (e & 3);
-                    const T *p = q + in.q_off[r] + col * E;
-                    if constexpr (FULL) rows_load(x, e, p); else rows_load_part(x, e, p, D - col * E);
-                    if (!whole && r0 + r >= rows) rows_clear(x, e);
-                }
-                const Frag<T> sf = frag_pack<T>(ds[0], ds[1]);
-#pragma unroll
-                for (int j = 0; j < E; j++) ak[j] = mma(rows_column(x, j), sf, ak[j]);
-            }
+        for (int x = 0; x < KW; x++) {
+            const int key = b * G.block + part * 64 + (kw * KW + x) * 16 + col;
+            if (key >= sq.k_len) continue;
+            const long long at = ((sq.k_base + key) * G.kv_heads + g) * G.head_dim;
+            store_row<T, DP>(dk + at, a.k[x], 1.f, quad, G.head_dim);
+            store_row<T, DP>(dv + at, a.v[x], 1.f, quad, G.head_dim);
         }
     }
-    if (mine) {
-        const long long at = (krow * G.kv_heads + g) * D;
+};
+
+template <class T, int DP, int KW, int KEYS, int ROWS>
+__global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>::kWaves))
+    k_attend_dkv(const Geometry G, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const T *__restrict__ dout,
+                 const RowInfo *__restrict__ rinfo, const unsigned long long *__restrict__ bits, const Item *__restrict__ items,
+                 const int *__restrict__ n_items, float *__restrict__ slots, T *__restrict__ dk, T *__restrict__ dv, int words, int parts, int per_item,
+                 unsigned group_inv)
+{
+    using C = Dkv<T, DP, KW, KEYS, ROWS>;
+    constexpr int KS = C::KS, E = C::E, kThreads = C::kThreads, kStep = C::kStep, kPieces = C::kPieces;
+    __shared__ u32x4 tiles[4 * C::kTile];
+    __shared__ int list[kListed];
+    __shared__ int listed, passed;
+    __shared__ long long still;
+    __shared__ __align__(16) float s_lse2[2][kStep], s_delta[2][kStep], s_inv[2][kStep];
+    __shared__ __align__(16) int s_limit[2][kStep];
+    const int tid = (int)threadIdx.x, lane = lane_id(), col = lane & 15, quad = lane >> 4;
+    const int wave = uniform(tid >> 6), kw = wave % KEYS, rw = wave / KEYS;
+    const auto qt = [&](int buf) { return tiles + buf * C::kTile; };
+    const auto gt = [&](int buf) { return tiles + (2 + buf) * C::kTile; };
+    const int part = (int)(blockIdx.x % parts);
+    Item it{(int)(blockIdx.x / parts), 0, 1, 0};
+    if (items) {
+        if (it.gm >= *n_items) return;
+        it = items[it.gm];
+    }
+    const int g = it.gm % G.kv_heads;
+    Seq sq;
+    int b;
+    if (!block_of_mean_row(G, it.gm / G.kv_heads, sq, b)) return;
+    const int D = G.head_dim;
+    const int key0 = b * G.block + part * 64 + kw * KW * 16 + col;  // inside the sequence; the wavefront's other keys are 16 further
+    if (b * G.block + part * 64 >= sq.k_len) return;
+    Frag<T> kf[KW][KS], vf[KW][KS];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int d = (4 * quad + e) * E;
-            float x[E];
+    for (int x = 0; x < KW; x++) {
+        const bool mine = key0 + 16 * x < sq.k_len;
+        const long long r = sq.k_base + (mine ? key0 + 16 * x : b * G.block);
+        row_frags<T, KS, false>(kf[x], k + r * G.k_row + (long long)g * G.k_head, quad, D, mine);
+        row_frags<T, KS, false>(vf[x], v + r * G.v_row + (long long)g * G.v_head, quad, D, mine);
+    }
+    typename C::Sums a;
 #pragma unroll
-            for (int j = 0; j < E; j++) x[j] = av[j][e];
-            store_columns<T, E>(dv + at + d, x, D - d);
+    for (int x = 0; x < KW; x++)
 #pragma unroll
-            for (int j = 0; j < E; j++) x[j] = ak[j][e];
-            store_columns<T, E>(dk + at + d, x, D - d);
+        for (int j = 0; j < E; j++) a.k[x][j] = a.v[x][j] = f32x4{0, 0, 0, 0};
+    const float sl2 = G.scale * kLog2e;
+    const unsigned long long *mybits = bits + (long long)it.gm * words;
+    int w0, w1;
+    words_of_block(G, sq, b, w0, w1);
+    long long skip = (long long)it.chunk * per_item, left = per_item;  // rows of the earlier items, rows of this one
+    for (int w = w0; w < w1 && left > 0;) {
+        // up to kListed rows of the item: 64 words at a time
+        __syncthreads();
+        if (wave == 0) {
+            const int lane = opaque(lane_id());
+            int have = 0, ww = w;
+            long long sk = skip;
+            const long long most = left < kListed ? left : kListed;
+            while (ww < w1 && have < most) {
+                unsigned long long m = ww + lane < w1 ? mybits[ww + lane] : 0;
+                const int n = __popcll(m);
+                int sum = n;
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) {
+                    const int o = pull(sum, lane - d);
+                    if (lane >= d) sum += o;
+                }
+                // words are taken whole: as many as fit
+                const bool fits = have + (sum - sk > 0 ? sum - sk : 0) <= kListed;
+                const int taken = __popcll(__ballot(fits && ww + lane < w1));
+                if (taken == 0) break;
+                long long at = (long long)have + sum - n - sk;  // place of the word's first row, negative where an earlier item has it
+                const int t0 = (ww + lane) * 64;
+                if (lane < taken)
+                    while (m) {
+                        if (at >= 0 && at < most) list[at] = t0 + __builtin_ctzll(m);
+                        at++;
+                        m &= m - 1;
+                    }
+                const int got = read_lane(sum, taken - 1);
+                const long long fresh = got - sk;
+                sk = fresh < 0 ? -fresh : 0;
+                have += fresh > 0 ? (int)fresh : 0;
+                ww += taken;
+            }
+            if (lane == 0) {
+                listed = have < most ? have : (int)most;
+                passed = ww;
+                still = sk;
+            }
         }
+        __syncthreads();
+        const int n = uniform(listed);
+        skip = (long long)uniform64((unsigned long long)still);
+        w = uniform(passed);
+        left -= n;
+        const int rows = n * G.group, steps = (rows + kStep - 1) / kStep;
+        // row r of the batch: token list[r / group], head r % group
+        auto token_of = [&](int r) { return group_inv ? (int)__umulhi((unsigned)r, group_inv) : r; };
+        auto prepare = [&](int step, int buf) {
+            const int o = opaque(tid);
+            const int r0 = step * kStep;
+            const bool whole = D == DP && r0 + kStep <= rows;
+#pragma unroll
+            for (int i = 0; i < C::kTile / kThreads; i++) {
+                const int x = i * kThreads + o, r = x / kPieces, rr = r0 + r;
+                const int c = ((x % kPieces) ^ (r & Tile<T, DP>::kSwizzle)) * Tile<T, DP>::kPer;
+                const bool in = rr < rows;
+                const int ti = token_of(in ? rr : 0), hh = g * G.group + ((in ? rr : 0) - ti * G.group);
+                const long long t = list[ti];
+                const T *pq = q + t * G.q_row + (long long)hh * G.q_head + c, *pg = dout + (t * G.heads + hh) * D + c;
+                if (whole) {
+                    const int base = i * kThreads + uniform(o & ~63);
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)pq,
+                                                     (__attribute__((address_space(3))) void *)(qt(buf) + base), 16, 0, 0);
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)pg,
+                                                     (__attribute__((address_space(3))) void *)(gt(buf) + base), 16, 0, 0);
+                } else {
+                    u32x4 y = u32x4{0, 0, 0, 0}, z = y;
+                    if (in && c < D) {
+                        y = *(const u32x4 *)pq;
+                        z = *(const u32x4 *)pg;
+                    }
+                    qt(buf)[x] = y;
+                    gt(buf)[x] = z;
+                }
+            }
+            if (o < kStep) {
+                const int rr = r0 + o;
+                RowInfo ri{INFINITY, 0.f, 1.f, 0.f};
+                int lim = 0;
+                if (rr < rows) {
+                    const int ti = token_of(rr);
+                    const long long t = list[ti];
+                    ri = rinfo[t * G.heads + g * G.group + (rr - ti * G.group)];
+                    lim = visible_keys(G, sq, (int)(t - sq.q_base));
+                }
+                s_lse2[buf][o] = ri.lse2;
+                s_delta[buf][o] = ri.delta;
+                if (sizeof(T) == 4) s_inv[buf][o] = ri.inv;
+                s_limit[buf][o] = lim;
+            }
+        };
+        if (steps > 0) prepare(0, 0);
+        __syncthreads();
+        for (int step = 0; step < steps; step++) {
+            const int buf = step & 1;
+            if (step + 1 < steps) prepare(step + 1, buf ^ 1);
+            const int base = 32 * rw;
+            if (step * kStep + base < rows) {
+                f32x4 s[KW][2], ds[KW][2];
+#pragma unroll
+                for (int x = 0; x < KW; x++) s[x][0] = s[x][1] = ds[x][0] = ds[x][1] = f32x4{0, 0, 0, 0};
+                pipelined<Frag<T>, 4 * KS, 4, 2>(
+                    [&](int i) { return tile_frag<T, DP>(i < 2 * KS ? qt(buf) : gt(buf), base + 16 * (i / KS & 1) + col, i % KS, quad); },
+                    [&](int i, const Frag<T> &f) {
+                        const int y = i / KS & 1;
+#pragma unroll
+                        for (int x = 0; x < KW; x++) {
+                            if (i < 2 * KS) s[x][y] = mma(f, kf[x][i % KS], s[x][y]);
+                            else ds[x][y] = mma(f, vf[x][i % KS], ds[x][y]);
+                        }
+                    });
+                Frag<T> pf[KW], df[KW];
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    const int r = base + 16 * y + 4 * quad;
+                    const f32x4 l2 = *(const f32x4 *)&s_lse2[buf][r], de = *(const f32x4 *)&s_delta[buf][r];
+                    typedef __attribute__((ext_vector_type(4))) int i32x4;
+                    const i32x4 li = *(const i32x4 *)&s_limit[buf][r];
+                    f32x4 iv = f32x4{1.f, 1.f, 1.f, 1.f};
+                    if (sizeof(T) == 4) iv = *(const f32x4 *)&s_inv[buf][r];
+#pragma unroll
+                    for (int x = 0; x < KW; x++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const bool on = key0 + 16 * x < li[e];
+                            float p = pow2(__builtin_fmaf(s[x][y][e], sl2, -l2[e]));
+                            if (sizeof(T) == 4) p *= iv[e];
+                            s[x][y][e] = on ? p : 0.f;
+                            ds[x][y][e] = on ? p * (ds[x][y][e] - de[e]) * G.scale : 0.f;
+                        }
+                }
+#pragma unroll
+                for (int x = 0; x < KW; x++) {
+                    pf[x] = frag_pack<T>(s[x][0], s[x][1]);
+                    df[x] = frag_pack<T>(ds[x][0], ds[x][1]);
+                }
+                if constexpr (sizeof(T) == 2) {
+                    pipelined<Frag<T>, 2 * E, 4, 2>(
+                        [&](int i) { return Columns<T, DP>(i < E ? gt(buf) : qt(buf), 2 * rw, quad, col).frag(i % E); },
+                        [&](int i, const Frag<T> &f) {
+#pragma unroll
+                            for (int x = 0; x < KW; x++) {
+                                if (i < E) a.v[x][i % E] = mma(f, pf[x], a.v[x][i % E]);
+                                else a.k[x][i % E] = mma(f, df[x], a.k[x][i % E]);
+                            }
+                        });
+                } else {
+                    {
+                        const Columns<T, DP> c(gt(buf), 2 * rw, quad, col);
+#pragma unroll
+                        for (int j = 0; j < E; j++)
+#pragma unroll
+                            for (int x = 0; x < KW; x++) a.v[x][j] = mma(c.frag(j), pf[x], a.v[x][j]);
+                    }
+                    {
+                        const Columns<T, DP> c(qt(buf), 2 * rw, quad, col);
+#pragma unroll
+                        for (int j = 0; j < E; j++)
+#pragma unroll
+                            for (int x = 0; x < KW; x++) a.k[x][j] = mma(c.frag(j), df[x], a.k[x][j]);
+                    }
+                }
+            }
+            __syncthreads();
+        }
+    }
+    // the wavefronts with other rows: added up in their order
+    if constexpr (ROWS > 1) {
+        float *ex = (float *)tiles;
+        static_assert((ROWS - 1) * KEYS * C::kDump * 64 * 4 <= (int)sizeof(tiles), "the exchange fits the tiles");
+        __syncthreads();
+        if (rw > 0) {
+#pragma unroll
+            for (int i = 0; i < C::kDump; i++) ex[(((rw - 1) * KEYS + kw) * C::kDump + i) * 64 + lane] = a.at(i);
+        }
+        __syncthreads();
+        if (rw > 0) return;
+#pragma unroll
+        for (int w = 0; w < ROWS - 1; w++)
+#pragma unroll
+            for (int i = 0; i < C::kDump; i++) a.at(i) += ex[((w * KEYS + kw) * C::kDump + i) * 64 + lane];
+    }
+    if (it.chunks > 1) {
+        float *p = slots + (((long long)it.slot * parts + part) * KEYS + kw) * C::kDump * 64 + lane;
+#pragma unroll
+        for (int i = 0; i < C::kDump; i++) p[i * 64] = a.at(i);
+    } else {
+        C::store(G, a, sq, b, g, part, kw, dk, dv);
     }
 }
 
+// Blocks of several items: the items' sums, added in their order.
+template <class T, int DP, int KW, int KEYS, int ROWS>
+__global__ void __launch_bounds__(64 * KEYS)
+    k_join_dkv(const Geometry G, const Item *__restrict__ items, const int *__restrict__ n_items, const float *__restrict__ slots, T *__restrict__ dk,
+               T *__restrict__ dv, int parts)
+{
+    using C = Dkv<T, DP, KW, KEYS, ROWS>;
+    const int part = (int)(blockIdx.x % parts), i = (int)(blockIdx.x / parts);
+    if (i >= *n_items) return;
+    const Item it = items[i];
+    if (it.chunks < 2 || it.chunk != 0) return;
+    Seq sq;
+    int b;
+    if (!block_of_mean_row(G, it.gm / G.kv_heads, sq, b) || b * G.block + part * 64 >= sq.k_len) return;
+    const int kw = uniform((int)(threadIdx.x >> 6)), lane = lane_id();
+    typename C::Sums a;
+    const float *p = slots + (((long long)it.slot * parts + part) * KEYS + kw) * C::kDump * 64 + lane;
+#pragma unroll
+    for (int x = 0; x < C::kDump; x++) a.at(x) = p[x * 64];
+    for (int c = 1; c < it.chunks; c++) {
+        p += (long long)parts * KEYS * C::kDump * 64;
+#pragma unroll
+        for (int x = 0; x < C::kDump; x++) a.at(x) += p[x * 64];
+    }
+    C::store(G, a, sq, b, it.gm % G.kv_heads, part, kw, dk, dv);
+}
+
+// What the backward pass keeps in the workspace.
 struct BwdSpace {
-    long long mean_rows, info_bytes, total;
-    int words;
+    long long gms, max_items, info_at, bits_at, chunks_at, items_at, slots_at, total;
+    int words, per_item, parts;
+    bool shared_out;  // some block may have more rows than an item
 };
 static BwdSpace bwd_space(const Geometry &G)
 {
     BwdSpace s;
-    s.mean_rows = G.cu_k ? G.k_rows / G.block + G.n_seq : (long long)G.blocks_each * G.n_seq;
+    const auto up = [](long long x) { return ceil_div(x, 256) * 256; };
+    s.gms = (G.cu_k ? G.k_rows / G.block + G.n_seq : (long long)G.blocks_each * G.n_seq) * G.kv_heads;
     s.words = (int)ceil_div(G.q_rows, 64);
-    s.info_bytes = ceil_div((long long)G.q_rows * G.heads * (long long)sizeof(RowInfo), 256) * 256;
-    s.total = s.info_bytes + 8 * (long long)G.kv_heads * s.mean_rows * s.words;
+    s.parts = G.block > 64 ? G.block / 64 : 1;
+    // items of at least 1024 rows, and not so many that their sums fill the memory: at most 8192 of them are kept
+    const long long listed = (long long)G.q_rows * G.kv_heads * G.width;
+    s.per_item = 1024;
+    while (listed / s.per_item > 4096) s.per_item *= 2;
+    s.shared_out = G.q_rows > s.per_item;
+    s.max_items = s.gms + (s.shared_out ? listed / s.per_item : 0);
+    // a block with n > per_item rows has at most 2 n / per_item items
+    const long long keep = s.shared_out ? 2 * (listed / s.per_item + 1) : 0;
+    const int dims = G.head_dim <= 64 ? 64 : G.head_dim <= 128 ? 128 : 256;
+    s.info_at = 0;
+    s.bits_at = up((long long)G.q_rows * G.heads * (long long)sizeof(RowInfo));
+    s.chunks_at = s.bits_at + up(8 * s.gms * s.words);
+    s.items_at = s.chunks_at + (s.shared_out ? up(4 * (s.gms + 1)) : 0);
+    s.slots_at = s.items_at + (s.shared_out ? up((long long)sizeof(Item) * s.max_items) : 0);
+    s.total = s.slots_at + keep * G.block * dims * 2 * 4;
     return s;
+}
+
+template <class T, int DP, int KW, int KEYS, int ROWS>
+static void launch_dkv(const Geometry &G, const void *q, const void *k, const void *v, const void *dout, void *dk, void *dv, char *ws,
+                       const BwdSpace &sp, hipStream_t st)
+{
+    const RowInfo *info = (const RowInfo *)(ws + sp.info_at);
+    const unsigned long long *bits = (const unsigned long long *)(ws + sp.bits_at);
+    const Item *items = sp.shared_out ? (const Item *)(ws + sp.items_at) : nullptr;
+    const int *n_items = (const int *)(ws + sp.chunks_at) + sp.gms;
+    float *slots = (float *)(ws + sp.slots_at);
+    // floor(r * inv / 2^32) = r / group for r < kListed * group <= 2^20: inv is off by less than group / 2^32 of 1 / group
+    const unsigned inv = G.group == 1 ? 0 : (unsigned)((0x100000000ULL + G.group - 1) / G.group);
+    hipLaunchKernelGGL((k_attend_dkv<T, DP, KW, KEYS, ROWS>), dim3((unsigned)(sp.max_items * sp.parts)), dim3(64 * KEYS * ROWS), 0, st, G,
+                       (const T *)q, (const T *)k, (const T *)v, (const T *)dout, info, bits, items, n_items, slots, (T *)dk, (T *)dv, sp.words,
+                       sp.parts, sp.per_item, inv);
+    if (sp.shared_out)
+        hipLaunchKernelGGL((k_join_dkv<T, DP, KW, KEYS, ROWS>), dim3((unsigned)(sp.max_items * sp.parts)), dim3(64 * KEYS), 0, st, G, items, n_items,
+                           slots, (T *)dk, (T *)dv, sp.parts);
 }
 
 template <class T, int DP, int NG>
 static void launch_bwd(const Geometry &G, const void *q, const void *k, const void *v, const int *idx, const void *out, const float *lse,
                        const void *dout, void *dq, void *dk, void *dv, char *ws, const BwdSpace &sp, hipStream_t st)
 {
-    RowInfo *info = (RowInfo *)ws;
-    unsigned long long *bits = (unsigned long long *)(ws + sp.info_bytes);
+    RowInfo *info = (RowInfo *)(ws + sp.info_at);
+    unsigned long long *bits = (unsigned long long *)(ws + sp.bits_at);
     const int slices = (int)ceil_div(G.group, 16);
-    const bool full = G.head_dim == DP;
     if (G.q_rows > 0) {
         const int per_tile = G.group < 16 ? 16 / G.group : 1;
 #define NSP_GO(NT, WIDE)                                                                                                                     \
@@ -451,20 +688,26 @@ static void launch_bwd(const Geometry &G, const void *q, const void *k, const vo
             if (G.block >= 16 * NG) NSP_GO(1, true); else NSP_GO(1, false);
         }
 #undef NSP_GO
-        if (sp.mean_rows > 0)
-            hipLaunchKernelGGL(k_pattern_bits, dim3((unsigned)((long long)sp.words * G.kv_heads)), dim3(256), 0, st, G, idx, bits,
-                               sp.mean_rows, sp.words);
+        if (sp.gms > 0) {
+            hipLaunchKernelGGL(k_pattern_bits, dim3((unsigned)((long long)sp.words * G.kv_heads)), dim3(256), 0, st, G, idx, bits, sp.words);
+            if (sp.shared_out) {
+                int *chunks = (int *)(ws + sp.chunks_at);
+                hipLaunchKernelGGL(k_count_chunks, dim3((unsigned)ceil_div(sp.gms, 4)), dim3(256), 0, st, G, bits, chunks, sp.gms, sp.words, sp.per_item);
+                hipLaunchKernelGGL(k_plan_items, dim3(1), dim3(1024), 0, st, chunks, sp.gms, (Item *)(ws + sp.items_at), chunks + sp.gms);
+            }
+        }
     }
-    if (sp.mean_rows > 0) {
-        const int parts = G.block > 64 ? G.block / 64 : 1;
-        const dim3 grid((unsigned)(sp.mean_rows * G.kv_heads * parts)), block(G.block > 64 ? 256 : 4 * G.block);
-        if (full)
-            hipLaunchKernelGGL((k_attend_dkv<T, DP, true>), grid, block, 0, st, G, (const T *)q, (const T *)k, (const T *)v,
-                               (const T *)dout, info, bits, (T *)dk, (T *)dv, sp.mean_rows, sp.words, parts);
-        else
-            hipLaunchKernelGGL((k_attend_dkv<T, DP, false>), grid, block, 0, st, G, (const T *)q, (const T *)k, (const T *)v,
-                               (const T *)dout, info, bits, (T *)dk, (T *)dv, sp.mean_rows, sp.words, parts);
-    }
+    if (sp.gms == 0) return;
+    // wavefronts over the keys x wavefronts over the rows, as the sums' registers and the tiles' LDS allow
+    constexpr int kKw = sizeof(T) == 2 && DP <= 128 ? 2 : 1;
+    constexpr int kMost = 128 * 1024 / (4 * 32 * DP * (int)sizeof(T));  // wavefronts over the rows that 128 KB hold tiles for
+    constexpr int kRows1 = kMost < 4 ? kMost : 4, kRows2 = kMost < 2 ? kMost : 2;
+    if (G.block == 16)
+        launch_dkv<T, DP, 1, 1, kRows1>(G, q, k, v, dout, dk, dv, ws, sp, st);
+    else if (G.block == 32)
+        launch_dkv<T, DP, kKw, 2 / kKw, kKw == 2 ? kRows1 : kRows2>(G, q, k, v, dout, dk, dv, ws, sp, st);
+    else
+        launch_dkv<T, DP, kKw, 4 / kKw, kKw == 2 ? kRows2 : 1>(G, q, k, v, dout, dk, dv, ws, sp, st);
 }
 
 }  // namespace lm
@@ -492,7 +735,7 @@ int nsparse_lm_block_attention_bwd(const nsparse_lm_attn *a, const void *q, cons
     if (int rc = geometry(a, true, true, &G)) return rc;
     if (G.page_size > 0) return fail(NSPARSE_LM_EARG, "block_attention_bwd: not for paged caches");
     const BwdSpace sp = bwd_space(G);
-    if (sp.mean_rows * G.kv_heads > 0x7fffffffLL / 4) return fail(NSPARSE_LM_EARG, "block_attention_bwd: blocks x heads out of range");
+    if (sp.max_items * sp.parts > 0x7fffffffLL || (long long)sp.words * G.kv_heads > 0x7fffffffLL) return fail(NSPARSE_LM_EARG, "block_attention_bwd: blocks x heads out of range");
     if ((G.q_rows > 0 && (!q || !idx || !out || !lse || !dout || !dq)) || (G.k_rows > 0 && (!k || !v || !dk || !dv)))
         return fail(NSPARSE_LM_EARG, "block_attention_bwd: a required pointer is NULL");
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv |
