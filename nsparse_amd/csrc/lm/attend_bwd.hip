@@ -253,35 +253,39 @@ __device__ inline void words_of_block(const Geometry &G, const Seq &sq, int b, i
     w1 = sq.q_len > i0 ? (int)((sq.q_base + sq.q_len - 1) >> 6) + 1 : w0;
 }
 
-// A block that many rows list (the first of a sequence, often) is shared out: an item is at most `per_item` of a block's rows.
+// A block's rows are shared out to items of at most `per_item`, all of a block nearly alike.
 struct Item {
-    int gm, chunk, chunks, slot;  // mean row * kv_heads + head; slot of the item's sums where the block has several
+    int gm, begin, count;     // mean row * kv_heads + head; which of the rows that list the block
+    int chunk, chunks, slot;  // of the block's items; where the item's sums go if there are several
 };
 __global__ void __launch_bounds__(256)
-    k_count_chunks(const Geometry G, const unsigned long long *__restrict__ bits, int *__restrict__ chunks, long long gms, int words, int per_item)
+    k_count_rows(const Geometry G, const unsigned long long *__restrict__ bits, int *__restrict__ counts, long long gms, int words)
 {
     const long long gm = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (gm >= gms) return;
     Seq sq;
     int b, n = 0, w0, w1;
     if (!block_of_mean_row(G, gm / G.kv_heads, sq, b)) {
-        if (lane_id() == 0) chunks[gm] = 0;
+        if (lane_id() == 0) counts[gm] = -1;
         return;
     }
     words_of_block(G, sq, b, w0, w1);
     for (int w = w0 + lane_id(); w < w1; w += 64) n += __popcll(bits[gm * words + w]);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
-    if (lane_id() == 0) chunks[gm] = n <= per_item ? 1 : (n + per_item - 1) / per_item;
+    if (lane_id() == 0) counts[gm] = n;
 }
-__global__ void __launch_bounds__(1024) k_plan_items(const int *__restrict__ chunks, long long gms, Item *__restrict__ items, int *__restrict__ n_items)
+__global__ void __launch_bounds__(1024)
+    k_plan_items(const int *__restrict__ counts, long long gms, int per_item, Item *__restrict__ items, int *__restrict__ n_items)
 {
     __shared__ int sums[2][16];
     const int lane = lane_id(), wave = (int)(threadIdx.x >> 6);
     int base = 0, slots = 0;
     for (long long g0 = 0; g0 < gms; g0 += 1024) {
         const long long gm = g0 + threadIdx.x;
-        const int n = gm < gms ? chunks[gm] : 0, m = n > 1 ? n : 0;
+        const int rows = gm < gms ? counts[gm] : -1;
+        // a block that no row lists is an item too: its gradients are zeros
+        const int n = rows < 0 ? 0 : rows <= per_item ? 1 : (rows + per_item - 1) / per_item, m = n > 1 ? n : 0;
         int a = n, c = m;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -305,7 +309,10 @@ __global__ void __launch_bounds__(1024) k_plan_items(const int *__restrict__ chu
             base += sums[0][w];
             slots += sums[1][w];
         }
-        for (int i = 0; i < n; i++) items[at + i] = Item{(int)gm, i, n, slot + i};
+        for (int i = 0; i < n; i++) {
+            const int x = (int)((long long)rows * i / n), y = (int)((long long)rows * (i + 1) / n);
+            items[at + i] = Item{(int)gm, x, y - x, i, n, slot + i};
+        }
         __syncthreads();
     }
     if (threadIdx.x == 0) *n_items = base;
@@ -315,20 +322,19 @@ __global__ void __launch_bounds__(1024) k_plan_items(const int *__restrict__ chu
 // An item's workgroup owns up to 64 keys of the block: KEYS wavefronts side by side with KW x 16 keys each, as the columns of their
 // products, and ROWS of them one behind the other, each with its own 32 of the (query, head) pairs that list the block.
 // The pairs' rows of q and dout go through LDS (by rows for S = Q K^T and dP = dO V^T, transposed for dK^T = Q^T dS and
-// dV^T = dO^T P), fetched while the 32 before are computed.  Bound by what LDS delivers: KW = 2 halves the reads a product.
+// dV^T = dO^T P), fetched while the 32 before are computed.  Bound by what LDS delivers: the more keys a wavefront, the fewer reads a product.
+#ifndef NSP_ITEMS
+#define NSP_ITEMS 1024
+#endif
 constexpr int kListed = 1024;
 template <class T, int DP, int KW, int KEYS, int ROWS> struct Dkv {
     static constexpr int KS = DP / 32, E = DP / 16, kThreads = 64 * KEYS * ROWS, kStep = 32 * ROWS;
     static constexpr int kPieces = Tile<T, DP>::kPieces, kTile = kStep * kPieces;
-    static constexpr int kDump = KW * 2 * E * 4;  // sums a lane
-    static constexpr int kWaves = DP * sizeof(T) <= 256 && kTile <= 1024 ? 2 : 1;  // a SIMD: what the sums and the tiles leave room for
+    static constexpr int kDump = KW * 2 * E;  // sums a lane, in fours
+    static constexpr int kWaves = DP * sizeof(T) > 256 ? 1 : KW == 1 && kTile <= 512 ? 3 : kTile <= 1024 ? 2 : 1;  // a SIMD: what the sums and the tiles leave room for
     struct Sums {
         f32x4 k[KW][E], v[KW][E];
-        __device__ inline float &at(int i)
-        {
-            f32x4 &x = i / 4 < KW * E ? k[i / 4 / E][i / 4 % E] : v[(i / 4 - KW * E) / E][i / 4 % E];
-            return ((float *)&x)[i & 3];
-        }
+        __device__ inline f32x4 &at(int i) { return i < KW * E ? k[i / E][i % E] : v[(i - KW * E) / E][i % E]; }
     };
     static __device__ inline void store(const Geometry &G, Sums &a, const Seq &sq, int b, int g, int part, int kw, T *dk, T *dv)
     {
@@ -348,7 +354,7 @@ template <class T, int DP, int KW, int KEYS, int ROWS>
 __global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>::kWaves))
     k_attend_dkv(const Geometry G, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const T *__restrict__ dout,
                  const RowInfo *__restrict__ rinfo, const unsigned long long *__restrict__ bits, const Item *__restrict__ items,
-                 const int *__restrict__ n_items, float *__restrict__ slots, T *__restrict__ dk, T *__restrict__ dv, int words, int parts, int per_item,
+                 const int *__restrict__ n_items, f32x4 *__restrict__ slots, T *__restrict__ dk, T *__restrict__ dv, int words, int parts,
                  unsigned group_inv)
 {
     using C = Dkv<T, DP, KW, KEYS, ROWS>;
@@ -364,7 +370,7 @@ __global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>:
     const auto qt = [&](int buf) { return tiles + buf * C::kTile; };
     const auto gt = [&](int buf) { return tiles + (2 + buf) * C::kTile; };
     const int part = (int)(blockIdx.x % parts);
-    Item it{(int)(blockIdx.x / parts), 0, 1, 0};
+    Item it{(int)(blockIdx.x / parts), 0, 0x7fffffff, 0, 1, 0};
     if (items) {
         if (it.gm >= *n_items) return;
         it = items[it.gm];
@@ -390,10 +396,11 @@ __global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>:
 #pragma unroll
         for (int j = 0; j < E; j++) a.k[x][j] = a.v[x][j] = f32x4{0, 0, 0, 0};
     const float sl2 = G.scale * kLog2e;
+    const int keys_end = sq.k_len < b * G.block + part * 64 + 64 ? sq.k_len : b * G.block + part * 64 + 64;
     const unsigned long long *mybits = bits + (long long)it.gm * words;
     int w0, w1;
     words_of_block(G, sq, b, w0, w1);
-    long long skip = (long long)it.chunk * per_item, left = per_item;  // rows of the earlier items, rows of this one
+    long long skip = it.begin, left = it.count;  // rows of the earlier items, rows of this one
     for (int w = w0; w < w1 && left > 0;) {
         // up to kListed rows of the item: 64 words at a time
         __syncthreads();
@@ -443,6 +450,29 @@ __global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>:
         const int rows = n * G.group, steps = (rows + kStep - 1) / kStep;
         // row r of the batch: token list[r / group], head r % group
         auto token_of = [&](int r) { return group_inv ? (int)__umulhi((unsigned)r, group_inv) : r; };
+        // what there is to know about a row is asked for before its tiles and put into LDS a step later: nothing waits for it
+        RowInfo ri;
+        int lim;
+        auto ask = [&](int step) {
+            const int o = opaque(tid), rr = step * kStep + o;
+            ri = RowInfo{INFINITY, 0.f, 1.f, 0.f};
+            lim = 0;
+            if (o < kStep && rr < rows) {
+                const int ti = token_of(rr);
+                const long long t = list[ti];
+                ri = rinfo[t * G.heads + g * G.group + (rr - ti * G.group)];
+                lim = visible_keys(G, sq, (int)(t - sq.q_base));
+            }
+        };
+        auto tell = [&](int buf) {
+            const int o = opaque(tid);
+            if (o < kStep) {
+                s_lse2[buf][o] = ri.lse2;
+                s_delta[buf][o] = ri.delta * G.scale;
+                if (sizeof(T) == 4) s_inv[buf][o] = ri.inv;
+                s_limit[buf][o] = lim;
+            }
+        };
         auto prepare = [&](int step, int buf) {
             const int o = opaque(tid);
             const int r0 = step * kStep;
@@ -471,66 +501,69 @@ __global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>:
                     gt(buf)[x] = z;
                 }
             }
-            if (o < kStep) {
-                const int rr = r0 + o;
-                RowInfo ri{INFINITY, 0.f, 1.f, 0.f};
-                int lim = 0;
-                if (rr < rows) {
-                    const int ti = token_of(rr);
-                    const long long t = list[ti];
-                    ri = rinfo[t * G.heads + g * G.group + (rr - ti * G.group)];
-                    lim = visible_keys(G, sq, (int)(t - sq.q_base));
-                }
-                s_lse2[buf][o] = ri.lse2;
-                s_delta[buf][o] = ri.delta;
-                if (sizeof(T) == 4) s_inv[buf][o] = ri.inv;
-                s_limit[buf][o] = lim;
-            }
         };
-        if (steps > 0) prepare(0, 0);
+        if (steps > 0) {
+            ask(0);
+            prepare(0, 0);
+            tell(0);
+        }
         __syncthreads();
         for (int step = 0; step < steps; step++) {
             const int buf = step & 1;
-            if (step + 1 < steps) prepare(step + 1, buf ^ 1);
+            if (step + 1 < steps) {
+                ask(step + 1);
+                prepare(step + 1, buf ^ 1);
+            }
             const int base = 32 * rw;
             if (step * kStep + base < rows) {
-                f32x4 s[KW][2], ds[KW][2];
-#pragma unroll
-                for (int x = 0; x < KW; x++) s[x][0] = s[x][1] = ds[x][0] = ds[x][1] = f32x4{0, 0, 0, 0};
-                pipelined<Frag<T>, 4 * KS, 4, 2>(
-                    [&](int i) { return tile_frag<T, DP>(i < 2 * KS ? qt(buf) : gt(buf), base + 16 * (i / KS & 1) + col, i % KS, quad); },
-                    [&](int i, const Frag<T> &f) {
-                        const int y = i / KS & 1;
-#pragma unroll
-                        for (int x = 0; x < KW; x++) {
-                            if (i < 2 * KS) s[x][y] = mma(f, kf[x][i % KS], s[x][y]);
-                            else ds[x][y] = mma(f, vf[x][i % KS], ds[x][y]);
-                        }
-                    });
                 Frag<T> pf[KW], df[KW];
+                // rows ascend, and so do the keys they see: the first row sees the fewest (rows that are not there see none)
+                const int fewest = uniform(s_limit[buf][base]), last = uniform(s_limit[buf][base + 31]);
+                const bool all = fewest >= keys_end && last >= keys_end;
 #pragma unroll
                 for (int y = 0; y < 2; y++) {
+                    f32x4 s[KW], ds[KW];
+#pragma unroll
+                    for (int x = 0; x < KW; x++) s[x] = ds[x] = f32x4{0, 0, 0, 0};
+                    pipelined<Frag<T>, 2 * KS, 4, 2>(
+                        [&](int i) { return tile_frag<T, DP>(i < KS ? qt(buf) : gt(buf), base + 16 * y + col, i % KS, quad); },
+                        [&](int i, const Frag<T> &f) {
+#pragma unroll
+                            for (int x = 0; x < KW; x++) {
+                                if (i < KS) s[x] = mma(f, kf[x][i % KS], s[x]);
+                                else ds[x] = mma(f, vf[x][i % KS], ds[x]);
+                            }
+                        });
                     const int r = base + 16 * y + 4 * quad;
                     const f32x4 l2 = *(const f32x4 *)&s_lse2[buf][r], de = *(const f32x4 *)&s_delta[buf][r];
-                    typedef __attribute__((ext_vector_type(4))) int i32x4;
-                    const i32x4 li = *(const i32x4 *)&s_limit[buf][r];
                     f32x4 iv = f32x4{1.f, 1.f, 1.f, 1.f};
                     if (sizeof(T) == 4) iv = *(const f32x4 *)&s_inv[buf][r];
 #pragma unroll
                     for (int x = 0; x < KW; x++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const bool on = key0 + 16 * x < li[e];
-                            float p = pow2(__builtin_fmaf(s[x][y][e], sl2, -l2[e]));
+                            float p = pow2(__builtin_fmaf(s[x][e], sl2, -l2[e]));
                             if (sizeof(T) == 4) p *= iv[e];
-                            s[x][y][e] = on ? p : 0.f;
-                            ds[x][y][e] = on ? p * (ds[x][y][e] - de[e]) * G.scale : 0.f;
+                            s[x][e] = p;
+                            ds[x][e] = p * __builtin_fmaf(ds[x][e], G.scale, -de[e]);
                         }
-                }
+                    if (!all) {
+                        typedef __attribute__((ext_vector_type(4))) int i32x4;
+                        const i32x4 li = *(const i32x4 *)&s_limit[buf][r];
 #pragma unroll
-                for (int x = 0; x < KW; x++) {
-                    pf[x] = frag_pack<T>(s[x][0], s[x][1]);
-                    df[x] = frag_pack<T>(ds[x][0], ds[x][1]);
+                        for (int x = 0; x < KW; x++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const bool on = key0 + 16 * x < li[e];
+                                s[x][e] = on ? s[x][e] : 0.f;
+                                ds[x][e] = on ? ds[x][e] : 0.f;
+                            }
+                    }
+#pragma unroll
+                    for (int x = 0; x < KW; x++) {
+                        frag_half(pf[x], y, s[x]);
+                        frag_half(df[x], y, ds[x]);
+                    }
                 }
                 if constexpr (sizeof(T) == 2) {
                     pipelined<Frag<T>, 2 * E, 4, 2>(
@@ -559,27 +592,34 @@ __global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>:
                     }
                 }
             }
+            if (step + 1 < steps) tell(buf ^ 1);
             __syncthreads();
         }
     }
     // the wavefronts with other rows: added up in their order
     if constexpr (ROWS > 1) {
-        float *ex = (float *)tiles;
-        static_assert((ROWS - 1) * KEYS * C::kDump * 64 * 4 <= (int)sizeof(tiles), "the exchange fits the tiles");
-        __syncthreads();
-        if (rw > 0) {
+        f32x4 *ex = (f32x4 *)tiles;
+        constexpr int kHalf = C::kDump / 2;  // dk's sums, then dv's
+        static_assert((ROWS - 1) * KEYS * kHalf * 64 * 16 <= (int)sizeof(tiles), "the exchange fits the tiles");
 #pragma unroll
-            for (int i = 0; i < C::kDump; i++) ex[(((rw - 1) * KEYS + kw) * C::kDump + i) * 64 + lane] = a.at(i);
+        for (int h = 0; h < 2; h++) {
+            __syncthreads();
+            if (rw > 0) {
+#pragma unroll
+                for (int i = 0; i < kHalf; i++) ex[(((rw - 1) * KEYS + kw) * kHalf + i) * 64 + lane] = a.at(h * kHalf + i);
+            }
+            __syncthreads();
+            if (rw == 0) {
+#pragma unroll
+                for (int w = 0; w < ROWS - 1; w++)
+#pragma unroll
+                    for (int i = 0; i < kHalf; i++) a.at(h * kHalf + i) += ex[((w * KEYS + kw) * kHalf + i) * 64 + lane];
+            }
         }
-        __syncthreads();
         if (rw > 0) return;
-#pragma unroll
-        for (int w = 0; w < ROWS - 1; w++)
-#pragma unroll
-            for (int i = 0; i < C::kDump; i++) a.at(i) += ex[((w * KEYS + kw) * C::kDump + i) * 64 + lane];
     }
     if (it.chunks > 1) {
-        float *p = slots + (((long long)it.slot * parts + part) * KEYS + kw) * C::kDump * 64 + lane;
+        f32x4 *p = slots + (((long long)it.slot * parts + part) * KEYS + kw) * C::kDump * 64 + lane;
 #pragma unroll
         for (int i = 0; i < C::kDump; i++) p[i * 64] = a.at(i);
     } else {
@@ -590,7 +630,7 @@ __global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>:
 // Blocks of several items: the items' sums, added in their order.
 template <class T, int DP, int KW, int KEYS, int ROWS>
 __global__ void __launch_bounds__(64 * KEYS)
-    k_join_dkv(const Geometry G, const Item *__restrict__ items, const int *__restrict__ n_items, const float *__restrict__ slots, T *__restrict__ dk,
+    k_join_dkv(const Geometry G, const Item *__restrict__ items, const int *__restrict__ n_items, const f32x4 *__restrict__ slots, T *__restrict__ dk,
                T *__restrict__ dv, int parts)
 {
     using C = Dkv<T, DP, KW, KEYS, ROWS>;
@@ -603,7 +643,7 @@ __global__ void __launch_bounds__(64 * KEYS)
     if (!block_of_mean_row(G, it.gm / G.kv_heads, sq, b) || b * G.block + part * 64 >= sq.k_len) return;
     const int kw = uniform((int)(threadIdx.x >> 6)), lane = lane_id();
     typename C::Sums a;
-    const float *p = slots + (((long long)it.slot * parts + part) * KEYS + kw) * C::kDump * 64 + lane;
+    const f32x4 *p = slots + (((long long)it.slot * parts + part) * KEYS + kw) * C::kDump * 64 + lane;
 #pragma unroll
     for (int x = 0; x < C::kDump; x++) a.at(x) = p[x * 64];
     for (int c = 1; c < it.chunks; c++) {
@@ -616,7 +656,7 @@ __global__ void __launch_bounds__(64 * KEYS)
 
 // What the backward pass keeps in the workspace.
 struct BwdSpace {
-    long long gms, max_items, info_at, bits_at, chunks_at, items_at, slots_at, total;
+    long long gms, max_items, info_at, bits_at, counts_at, items_at, slots_at, total;
     int words, per_item, parts;
     bool shared_out;  // some block may have more rows than an item
 };
@@ -627,10 +667,10 @@ static BwdSpace bwd_space(const Geometry &G)
     s.gms = (G.cu_k ? G.k_rows / G.block + G.n_seq : (long long)G.blocks_each * G.n_seq) * G.kv_heads;
     s.words = (int)ceil_div(G.q_rows, 64);
     s.parts = G.block > 64 ? G.block / 64 : 1;
-    // items of at least 1024 rows, and not so many that their sums fill the memory: at most 8192 of them are kept
+    // about 1024 items besides the blocks' own, of at least 64 rows
     const long long listed = (long long)G.q_rows * G.kv_heads * G.width;
-    s.per_item = 1024;
-    while (listed / s.per_item > 4096) s.per_item *= 2;
+    s.per_item = 64;
+    while (listed / s.per_item > NSP_ITEMS) s.per_item *= 2;
     s.shared_out = G.q_rows > s.per_item;
     s.max_items = s.gms + (s.shared_out ? listed / s.per_item : 0);
     // a block with n > per_item rows has at most 2 n / per_item items
@@ -638,8 +678,8 @@ static BwdSpace bwd_space(const Geometry &G)
     const int dims = G.head_dim <= 64 ? 64 : G.head_dim <= 128 ? 128 : 256;
     s.info_at = 0;
     s.bits_at = up((long long)G.q_rows * G.heads * (long long)sizeof(RowInfo));
-    s.chunks_at = s.bits_at + up(8 * s.gms * s.words);
-    s.items_at = s.chunks_at + (s.shared_out ? up(4 * (s.gms + 1)) : 0);
+    s.counts_at = s.bits_at + up(8 * s.gms * s.words);
+    s.items_at = s.counts_at + (s.shared_out ? up(4 * (s.gms + 1)) : 0);
     s.slots_at = s.items_at + (s.shared_out ? up((long long)sizeof(Item) * s.max_items) : 0);
     s.total = s.slots_at + keep * G.block * dims * 2 * 4;
     return s;
@@ -652,13 +692,13 @@ static void launch_dkv(const Geometry &G, const void *q, const void *k, const vo
     const RowInfo *info = (const RowInfo *)(ws + sp.info_at);
     const unsigned long long *bits = (const unsigned long long *)(ws + sp.bits_at);
     const Item *items = sp.shared_out ? (const Item *)(ws + sp.items_at) : nullptr;
-    const int *n_items = (const int *)(ws + sp.chunks_at) + sp.gms;
-    float *slots = (float *)(ws + sp.slots_at);
+    const int *n_items = (const int *)(ws + sp.counts_at) + sp.gms;
+    f32x4 *slots = (f32x4 *)(ws + sp.slots_at);
     // floor(r * inv / 2^32) = r / group for r < kListed * group <= 2^20: inv is off by less than group / 2^32 of 1 / group
     const unsigned inv = G.group == 1 ? 0 : (unsigned)((0x100000000ULL + G.group - 1) / G.group);
     hipLaunchKernelGGL((k_attend_dkv<T, DP, KW, KEYS, ROWS>), dim3((unsigned)(sp.max_items * sp.parts)), dim3(64 * KEYS * ROWS), 0, st, G,
                        (const T *)q, (const T *)k, (const T *)v, (const T *)dout, info, bits, items, n_items, slots, (T *)dk, (T *)dv, sp.words,
-                       sp.parts, sp.per_item, inv);
+                       sp.parts, inv);
     if (sp.shared_out)
         hipLaunchKernelGGL((k_join_dkv<T, DP, KW, KEYS, ROWS>), dim3((unsigned)(sp.max_items * sp.parts)), dim3(64 * KEYS), 0, st, G, items, n_items,
                            slots, (T *)dk, (T *)dv, sp.parts);
@@ -691,23 +731,24 @@ static void launch_bwd(const Geometry &G, const void *q, const void *k, const vo
         if (sp.gms > 0) {
             hipLaunchKernelGGL(k_pattern_bits, dim3((unsigned)((long long)sp.words * G.kv_heads)), dim3(256), 0, st, G, idx, bits, sp.words);
             if (sp.shared_out) {
-                int *chunks = (int *)(ws + sp.chunks_at);
-                hipLaunchKernelGGL(k_count_chunks, dim3((unsigned)ceil_div(sp.gms, 4)), dim3(256), 0, st, G, bits, chunks, sp.gms, sp.words, sp.per_item);
-                hipLaunchKernelGGL(k_plan_items, dim3(1), dim3(1024), 0, st, chunks, sp.gms, (Item *)(ws + sp.items_at), chunks + sp.gms);
+                int *counts = (int *)(ws + sp.counts_at);
+                hipLaunchKernelGGL(k_count_rows, dim3((unsigned)ceil_div(sp.gms, 4)), dim3(256), 0, st, G, bits, counts, sp.gms, sp.words);
+                hipLaunchKernelGGL(k_plan_items, dim3(1), dim3(1024), 0, st, counts, sp.gms, sp.per_item, (Item *)(ws + sp.items_at), counts + sp.gms);
             }
         }
     }
     if (sp.gms == 0) return;
-    // wavefronts over the keys x wavefronts over the rows, as the sums' registers and the tiles' LDS allow
-    constexpr int kKw = sizeof(T) == 2 && DP <= 128 ? 2 : 1;
+    // Keys a wavefront, then wavefronts over the keys x over the rows, as the sums' registers and the tiles' LDS allow.
+    constexpr int kWide = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
     constexpr int kMost = 128 * 1024 / (4 * 32 * DP * (int)sizeof(T));  // wavefronts over the rows that 128 KB hold tiles for
-    constexpr int kRows1 = kMost < 4 ? kMost : 4, kRows2 = kMost < 2 ? kMost : 2;
+    constexpr int kKw2 = kWide < 2 ? 1 : 2, kKeys2 = 2 / kKw2, kKeys4 = 4 / kWide;
+    constexpr int kRows1 = kMost < 4 ? kMost : 4, kRows2 = kMost < 4 / kKeys2 ? kMost : 4 / kKeys2, kRows4 = kMost < 4 / kKeys4 ? kMost : 4 / kKeys4;
     if (G.block == 16)
         launch_dkv<T, DP, 1, 1, kRows1>(G, q, k, v, dout, dk, dv, ws, sp, st);
     else if (G.block == 32)
-        launch_dkv<T, DP, kKw, 2 / kKw, kKw == 2 ? kRows1 : kRows2>(G, q, k, v, dout, dk, dv, ws, sp, st);
+        launch_dkv<T, DP, kKw2, kKeys2, kRows2>(G, q, k, v, dout, dk, dv, ws, sp, st);
     else
-        launch_dkv<T, DP, kKw, 4 / kKw, kKw == 2 ? kRows2 : 1>(G, q, k, v, dout, dk, dv, ws, sp, st);
+        launch_dkv<T, DP, kWide, kKeys4, kRows4>(G, q, k, v, dout, dk, dv, ws, sp, st);
 }
 
 }  // namespace lm

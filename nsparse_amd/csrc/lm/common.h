@@ -111,6 +111,17 @@ template <class T> __device__ inline Frag<T> frag_pack(f32x4 a, f32x4 b)
 }
 template <> __device__ inline Frag<float> frag_pack<float>(f32x4 a, f32x4 b) { return Frag<float>{a, b}; }
 
+// the same, half by half
+template <class T> __device__ inline void frag_half(Frag<T> &f, int h, f32x4 a)
+{
+    f.r[2 * h] = pack2(a[0], a[1], T{});
+    f.r[2 * h + 1] = pack2(a[2], a[3], T{});
+}
+template <> __device__ inline void frag_half<float>(Frag<float> &f, int h, f32x4 a)
+{
+    if (h == 0) f.lo = a; else f.hi = a;
+}
+
 // ---- a lane's share of 8 rows x E columns, and the E fragments of its transpose --------------------------------------
 // Lane (quad, r) loads, of each of its quad's eight slot rows, the E = DP / 16 neighbouring columns r * E ..: a row is read
 // by 16 lanes in one piece.  Fragment j of the transpose has column r * E + j as its row: which column a product's
