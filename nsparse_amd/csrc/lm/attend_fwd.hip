@@ -382,14 +382,16 @@ static void launch_attend(const Geometry &G, const void *q, const void *k, const
     const bool split = rows * G.kv_heads < 2048;
     const bool full = G.head_dim == DP;
     if (!split && G.q_rows / G.n_seq >= 4) {
+        // 64 keys a step where a block has them, else 32 (blocks of 32 in steps of 64: 58 against 39 us for 3945 rows of 16 heads)
+        const int per_tile = G.group < 16 ? 16 / G.group : 1;
         if constexpr (sizeof(T) == 2 && DP <= 128) {
-            const int per_tile = G.group < 16 ? 16 / G.group : 1;
-            if (per_tile <= 8 && rows * G.kv_heads >= 2 * per_tile * 2048LL) {
-                launch_tiles<T, DP, 2, NG>(G, q, k, v, idx, out, lse, st);
+            if (G.block >= 64) {
+                if (per_tile <= 8 && rows * G.kv_heads >= 2 * per_tile * 2048LL) launch_tiles<T, DP, 2, 4>(G, q, k, v, idx, out, lse, st);
+                else launch_tiles<T, DP, 1, 4>(G, q, k, v, idx, out, lse, st);
                 return;
             }
         }
-        launch_tiles<T, DP, 1, NG>(G, q, k, v, idx, out, lse, st);
+        launch_tiles<T, DP, 1, 2>(G, q, k, v, idx, out, lse, st);
         return;
     }
 #define NSP_GO(FULL, WAVES)                                                                                                          \

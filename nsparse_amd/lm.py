@@ -9,6 +9,7 @@ into a graph.  Refused arguments raise ValueError with the reason.  There is no 
 """
 import ctypes as C
 import math
+import struct
 
 import torch
 
@@ -39,6 +40,13 @@ class Seqs:
             raise ValueError("Seqs: page_table must be an int32 tensor [n, pages] with contiguous rows")
         self.cu_q, self.cu_k, self.q_len, self.k_len, self.page_table = cu_q, cu_k, q_len, k_len, page_table
 
+    # addresses, read at every call (0: none)
+    ptr_cu_q = property(lambda self: 0 if self.cu_q is None else self.cu_q.data_ptr())
+    ptr_cu_k = property(lambda self: 0 if self.cu_k is None else self.cu_k.data_ptr())
+    ptr_q_len = property(lambda self: 0 if self.q_len is None else self.q_len.data_ptr())
+    ptr_k_len = property(lambda self: 0 if self.k_len is None else self.k_len.data_ptr())
+    ptr_table = property(lambda self: 0 if self.page_table is None else self.page_table.data_ptr())
+
     def _tensors(self):
         return [t for t in (self.cu_q, self.cu_k, self.q_len, self.k_len, self.page_table) if t is not None]
 
@@ -54,13 +62,26 @@ def _check(rc):
 
 
 def _on_gpu(*tensors):
-    dev = tensors[0].device
-    if dev.type != "cuda":
+    """The index of the GPU that all tensors live on."""
+    dev = tensors[0].get_device()
+    if dev < 0:
         raise ValueError("tensors must live on a GPU")
     for t in tensors:
-        if t.device != dev:
+        if t.get_device() != dev:
             raise ValueError("all tensors must live on one device")
     return dev
+
+
+def _queued(dev, fn, *args):
+    """fn(*args, stream) with the tensors' device current."""
+    if torch.cuda.current_device() == dev:
+        return fn(*args, _raw_stream(dev))
+    with torch.cuda.device(dev):
+        return fn(*args, _raw_stream(dev))
+
+
+def _raw_stream(dev):
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _ptr(t):
@@ -68,75 +89,57 @@ def _ptr(t):
 
 
 def _contiguous(t, what, dtype=None, shape=None):
-    if not t.is_contiguous() or (dtype is not None and t.dtype != dtype) or (shape is not None and tuple(t.shape) != tuple(shape)):
+    if not t.is_contiguous() or (dtype is not None and t.dtype != dtype) or (shape is not None and t.shape != shape):
         raise ValueError(f"{what} must be contiguous" + (f", {dtype}" if dtype is not None else "") +
                          (f", of shape {tuple(shape)}" if shape is not None else ""))
 
 
-def _attn(seqs, block, *, q=None, k=None, v=None, q_heads=None, k_rows=None, width=1, causal=True, scale=0.0, first=0, local=0):
-    """The argument block of a call."""
-    a = LmAttn()
-    some = k if k is not None else q
-    if some.dtype not in _DTYPES:
+# the fields of LmAttn in their order (an int of padding before the 64-bit ones is the struct module's)
+_ATTN = struct.Struct("@11if3q5P8q")
+assert _ATTN.size == C.sizeof(LmAttn)
+
+
+def _attn(seqs, block, *, q=None, k=None, v=None, kv_heads=None, k_rows=None, page_size=0, width=1, causal=True, scale=0.0, first=0, local=0):
+    """The argument block of a call, and its key heads.  Without q: for the keys alone."""
+    some = q if k is None else k
+    dtype = _DTYPES.get(some.dtype)
+    if dtype is None:
         raise ValueError("tensors must be float32, float16 or bfloat16")
-    a.dtype = _DTYPES[some.dtype]
-    a.block, a.width, a.causal, a.n_seq = int(block), int(width), int(bool(causal)), seqs.n
-    a.first, a.local, a.scale = int(first), int(local), float(scale)
-    paged = seqs.page_table is not None
+    table = seqs.page_table
+    q_rows = heads = dim = q0 = q1 = 0
     if q is not None:
         if q.dim() != 3 or q.stride(2) != 1 and q.shape[2] > 1:
             raise ValueError("q must be [rows, heads, head_dim] with a contiguous head_dim")
-        a.q_rows, a.heads, a.head_dim = q.shape
-        a.q_stride[0], a.q_stride[1] = q.stride(0) if q.shape[0] > 1 else 0, q.stride(1) if q.shape[1] > 1 else 0
-        a.kv_heads = a.heads
+        q_rows, heads, dim = q.shape
+        q0, q1 = (q.stride(0) if q_rows > 1 else 0), (q.stride(1) if heads > 1 else 0)
+    ks = vs = (0, 0, 0)
     if k is not None:
-        for t, what in ((k, "k"), (v, "v")):
-            if t is None:
-                continue
-            if t.dim() != (4 if paged else 3) or t.stride(-1) != 1 and t.shape[-1] > 1:
-                raise ValueError(f"{what} must be [rows, kv_heads, head_dim], or [pages, page_size, kv_heads, head_dim] with a page table, "
-                                 "with a contiguous head_dim")
-            if t.shape != k.shape or t.dtype != k.dtype:
+        ks = _key_strides(k, "k", table is not None)
+        if v is not None:
+            if v.shape != k.shape or v.dtype != k.dtype:
                 raise ValueError("k and v must have one shape and type")
-        a.k_rows, a.kv_heads = k.shape[0], k.shape[-2]
+            vs = _key_strides(v, "v", table is not None)
+        shape = k.shape
+        k_rows, kv_heads = shape[0], shape[-2]
         if q is None:
-            a.heads, a.head_dim = a.kv_heads, k.shape[-1]
-            if not paged and seqs.cu_q is None:
-                a.q_rows = 0
-        elif q.shape[2] != k.shape[-1] or q.dtype != k.dtype:
+            heads, dim = kv_heads, shape[-1]
+        elif dim != shape[-1] or q.dtype != k.dtype:
             raise ValueError("q, k and v must have one head_dim and type")
-        if paged:
-            a.page_size = k.shape[1]
-        for t, stride in ((k, a.k_stride), (v, a.v_stride)):
-            if t is not None:
-                if paged:
-                    stride[0] = t.stride(0) if t.shape[0] > 1 else 0
-                stride[1] = t.stride(-3) if t.shape[-3] > 1 else 0
-                stride[2] = t.stride(-2) if t.shape[-2] > 1 else 0
-    if k_rows is not None:
-        a.k_rows = int(k_rows)
-    if q_heads is not None:
-        a.heads, a.kv_heads = q_heads
-    if paged:
-        a.table_stride = seqs.page_table.stride(0) if seqs.n > 1 else seqs.page_table.shape[1]
-    a.cu_q, a.cu_k, a.q_len, a.k_len, a.page_table = (_ptr(seqs.cu_q), _ptr(seqs.cu_k), _ptr(seqs.q_len), _ptr(seqs.k_len),
-                                                      _ptr(seqs.page_table))
-    return a
+        if table is not None:
+            page_size = shape[1]
+    a = LmAttn.from_buffer_copy(_ATTN.pack(
+        dtype, heads, kv_heads, dim, int(block), int(width), 1 if causal else 0, seqs.n, page_size, int(first), int(local), scale, q_rows,
+        int(k_rows), 0 if table is None else (table.stride(0) if seqs.n > 1 else table.shape[1]), 0 if q is None else seqs.ptr_cu_q,
+        seqs.ptr_cu_k, 0 if q is None else seqs.ptr_q_len, seqs.ptr_k_len, seqs.ptr_table, q0, q1, *ks, *vs))
+    return a, kv_heads
 
 
-class _Queue:
-    """The device of a call made current, and its current stream."""
-
-    def __init__(self, dev):
-        self.guard = torch.cuda.device(dev)
-        self.dev = dev
-
-    def __enter__(self):
-        self.guard.__enter__()
-        return torch.cuda.current_stream(self.dev).cuda_stream
-
-    def __exit__(self, *exc):
-        return self.guard.__exit__(*exc)
+def _key_strides(t, what, paged):
+    if t.dim() != (4 if paged else 3) or t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{what} must be [rows, kv_heads, head_dim], or [pages, page_size, kv_heads, head_dim] with a page table, "
+                         "with a contiguous head_dim")
+    shape, stride = t.shape, t.stride()
+    return (stride[0] if paged and shape[0] > 1 else 0, stride[-3] if shape[-3] > 1 else 0, stride[-2] if shape[-2] > 1 else 0)
 
 
 def _empty_or_zeros(whole, *shape, dtype, device):
@@ -153,21 +156,18 @@ def block_means(k, *, block, seqs=None, last=0, out=None):
     """
     seqs = seqs or _ONE
     dev = _on_gpu(k, *seqs._tensors(), *([out] if out is not None else []))
-    a = _attn(seqs, block, k=k)
-    a.cu_q = None
-    a.q_len = None
-    a.q_rows = 0
+    a, _ = _attn(seqs, block, k=k)
     lib = load_lm()
-    rows = lib.nsparse_lm_mean_rows(C.byref(a))
+    ref = C.byref(a)
+    rows = lib.nsparse_lm_mean_rows(ref)
     _check(min(rows, 0))
     shape = (rows, k.shape[-2], k.shape[-1])
     if out is None:
         whole = seqs.cu_k is None and seqs.k_len is None and last == 0
-        out = _empty_or_zeros(whole, *shape, dtype=k.dtype, device=dev)
+        out = _empty_or_zeros(whole, *shape, dtype=k.dtype, device=k.device)
     else:
         _contiguous(out, "out", k.dtype, shape)
-    with _Queue(dev) as st:
-        _check(lib.nsparse_lm_block_means(C.byref(a), _ptr(k), _ptr(out), int(last), st))
+    _check(_queued(dev, lib.nsparse_lm_block_means, ref, k.data_ptr(), out.data_ptr(), int(last)))
     return out
 
 
@@ -182,49 +182,50 @@ def select_blocks(q, means, *, block, width, k_rows, first=1, local=1, causal=Tr
     if means.dim() != 3 or means.dtype != q.dtype or means.shape[2] != q.shape[-1]:
         raise ValueError("means must be [rows, kv_heads, head_dim] in q's type")
     _contiguous(means, "means")
-    a = _attn(seqs, block, q=q, k_rows=k_rows, width=width, causal=causal, first=first, local=local)
-    a.kv_heads = means.shape[1]
-    lib = load_lm()
+    page_size = 0
     if seqs.page_table is not None:
         if k_rows < 1 or means.shape[0] % k_rows:
             raise ValueError("means must have page_size / block rows a page")
-        a.page_size = means.shape[0] // k_rows * int(block)
-    rows = lib.nsparse_lm_mean_rows(C.byref(a))
+        page_size = means.shape[0] // k_rows * int(block)
+    a, _ = _attn(seqs, block, q=q, kv_heads=means.shape[1], k_rows=k_rows, page_size=page_size, width=width, causal=causal, first=first, local=local)
+    lib = load_lm()
+    ref = C.byref(a)
+    rows = lib.nsparse_lm_mean_rows(ref)
     _check(min(rows, 0))
     if rows != means.shape[0]:
         raise ValueError(f"means must have {rows} rows for these keys")
     shape = (q.shape[0], means.shape[1], int(width))
     if out is None:
         whole = seqs.cu_q is None and seqs.q_len is None
-        out = torch.empty(shape, dtype=torch.int32, device=dev) if whole else torch.full(shape, -1, dtype=torch.int32, device=dev)
+        out = torch.empty(shape, dtype=torch.int32, device=q.device) if whole else torch.full(shape, -1, dtype=torch.int32, device=q.device)
     else:
         _contiguous(out, "out", torch.int32, shape)
-    with _Queue(dev) as st:
-        _check(lib.nsparse_lm_select_blocks(C.byref(a), _ptr(q), _ptr(means), _ptr(out), st))
+    _check(_queued(dev, lib.nsparse_lm_select_blocks, ref, q.data_ptr(), means.data_ptr(), out.data_ptr()))
     return out
 
 
-def _attention(q, k, v, idx, block, scale, causal, seqs, out, lse):
-    a = _attn(seqs, block, q=q, k=k, v=v, width=idx.shape[-1] if idx.dim() == 3 else 0, causal=causal, scale=scale)
-    _contiguous(idx, "idx", torch.int32, (q.shape[0], a.kv_heads, a.width))
+def _attention(dev, q, k, v, idx, block, scale, causal, seqs, out, lse):
+    a, kv_heads = _attn(seqs, block, q=q, k=k, v=v, width=idx.shape[-1] if idx.dim() == 3 else 0, causal=causal, scale=scale)
+    shape = q.shape
+    _contiguous(idx, "idx", torch.int32, (shape[0], kv_heads, a.width))
     whole = seqs.cu_q is None and seqs.q_len is None
     if out is None:
-        out = _empty_or_zeros(whole, *q.shape, dtype=q.dtype, device=q.device)
+        out = _empty_or_zeros(whole, *shape, dtype=q.dtype, device=q.device)
     else:
-        _contiguous(out, "out", q.dtype, q.shape)
+        _contiguous(out, "out", q.dtype, shape)
     if lse is None:
-        lse = _empty_or_zeros(whole, q.shape[0], q.shape[1], dtype=torch.float32, device=q.device)
+        lse = _empty_or_zeros(whole, shape[0], shape[1], dtype=torch.float32, device=q.device)
     else:
-        _contiguous(lse, "lse", torch.float32, q.shape[:2])
-    with _Queue(q.device) as st:
-        _check(load_lm().nsparse_lm_block_attention(C.byref(a), _ptr(q), _ptr(k), _ptr(v), _ptr(idx), _ptr(out), _ptr(lse), st))
+        _contiguous(lse, "lse", torch.float32, shape[:2])
+    _check(_queued(dev, load_lm().nsparse_lm_block_attention, C.byref(a), q.data_ptr(), k.data_ptr(), v.data_ptr(), idx.data_ptr(),
+                   out.data_ptr(), lse.data_ptr()))
     return out, lse
 
 
 class _BlockAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, idx, block, scale, causal, seqs):
-        out, lse = _attention(q, k, v, idx, block, scale, causal, seqs, None, None)
+        out, lse = _attention(q.get_device(), q, k, v, idx, block, scale, causal, seqs, None, None)
         ctx.save_for_backward(q, k, v, idx, out, lse, *seqs._tensors())
         ctx.rest = (block, scale, causal, seqs)
         ctx.mark_non_differentiable(lse)
@@ -246,7 +247,7 @@ def block_attention(q, k, v, idx, *, block, scale=None, causal=True, seqs=None, 
     returns it.  Differentiable in q, k, v (not over a paged cache).  out, lse: buffers to write into (then not differentiable).
     """
     seqs = seqs or _ONE
-    _on_gpu(q, k, v, idx, *seqs._tensors(), *[t for t in (out, lse) if t is not None])
+    dev = _on_gpu(q, k, v, idx, *seqs._tensors(), *[t for t in (out, lse) if t is not None])
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         if out is not None or lse is not None:
@@ -255,7 +256,7 @@ def block_attention(q, k, v, idx, *, block, scale=None, causal=True, seqs=None, 
             raise ValueError("a paged cache has no gradient")
         o, s = _BlockAttention.apply(q, k, v, idx, block, scale, causal, seqs)
     else:
-        o, s = _attention(q, k, v, idx, block, scale, causal, seqs, out, lse)
+        o, s = _attention(dev, q, k, v, idx, block, scale, causal, seqs, out, lse)
     return (o, s) if return_lse else o
 
 
@@ -264,23 +265,24 @@ def block_attention_backward(dout, q, k, v, idx, out, lse, *, block, scale=None,
     seqs = seqs or _ONE
     dev = _on_gpu(dout, q, k, v, idx, out, lse, *seqs._tensors())
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
-    a = _attn(seqs, block, q=q, k=k, v=v, width=idx.shape[-1] if idx.dim() == 3 else 0, causal=causal, scale=scale)
-    _contiguous(idx, "idx", torch.int32, (q.shape[0], a.kv_heads, a.width))
-    _contiguous(dout, "dout", q.dtype, q.shape)
-    _contiguous(out, "out", q.dtype, q.shape)
-    _contiguous(lse, "lse", torch.float32, q.shape[:2])
+    a, kv_heads = _attn(seqs, block, q=q, k=k, v=v, width=idx.shape[-1] if idx.dim() == 3 else 0, causal=causal, scale=scale)
+    shape = q.shape
+    _contiguous(idx, "idx", torch.int32, (shape[0], kv_heads, a.width))
+    _contiguous(dout, "dout", q.dtype, shape)
+    _contiguous(out, "out", q.dtype, shape)
+    _contiguous(lse, "lse", torch.float32, shape[:2])
     lib = load_lm()
-    need = lib.nsparse_lm_block_attention_bwd_workspace(C.byref(a))
+    ref = C.byref(a)
+    need = lib.nsparse_lm_block_attention_bwd_workspace(ref)
     _check(min(need, 0))
     whole_q = seqs.cu_q is None and seqs.q_len is None
     whole_k = seqs.cu_k is None and seqs.k_len is None
-    dq = _empty_or_zeros(whole_q, *q.shape, dtype=q.dtype, device=dev)
-    dk = _empty_or_zeros(whole_k, *k.shape, dtype=q.dtype, device=dev)
-    dv = _empty_or_zeros(whole_k, *k.shape, dtype=q.dtype, device=dev)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    with _Queue(dev) as st:
-        _check(lib.nsparse_lm_block_attention_bwd(C.byref(a), _ptr(q), _ptr(k), _ptr(v), _ptr(idx), _ptr(out), _ptr(lse), _ptr(dout),
-                                                  _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), need, st))
+    dq = _empty_or_zeros(whole_q, *shape, dtype=q.dtype, device=q.device)
+    dk = _empty_or_zeros(whole_k, *k.shape, dtype=q.dtype, device=q.device)
+    dv = _empty_or_zeros(whole_k, *k.shape, dtype=q.dtype, device=q.device)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _check(_queued(dev, lib.nsparse_lm_block_attention_bwd, ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), idx.data_ptr(), out.data_ptr(),
+                   lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), need))
     return dq, dk, dv
 
 
@@ -304,12 +306,12 @@ def route(ids, experts):
     tokens, top = ids.shape
     need = lib.nsparse_lm_route_workspace(tokens, top, int(experts))
     _check(min(need, 0))
-    offsets = torch.empty(int(experts) + 1, dtype=torch.int32, device=dev)
-    order = torch.empty(tokens * top, dtype=torch.int32, device=dev)
-    place = torch.empty(tokens, top, dtype=torch.int32, device=dev)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    with _Queue(dev) as st:
-        _check(lib.nsparse_lm_route(_ptr(ids), tokens, top, int(experts), _ptr(offsets), _ptr(order), _ptr(place), _ptr(ws), need, st))
+    offsets = torch.empty(int(experts) + 1, dtype=torch.int32, device=ids.device)
+    order = torch.empty(tokens * top, dtype=torch.int32, device=ids.device)
+    place = torch.empty(tokens, top, dtype=torch.int32, device=ids.device)
+    ws = torch.empty(need, dtype=torch.uint8, device=ids.device) if need else None
+    _check(_queued(dev, lib.nsparse_lm_route, ids.data_ptr(), tokens, top, int(experts), offsets.data_ptr(), order.data_ptr(), place.data_ptr(),
+                   _ptr(ws), need))
     return Route(offsets, order, place)
 
 
@@ -329,9 +331,9 @@ def _weights(w, plan):
 def _gather(x, plan):
     dev = _on_gpu(x, plan.place)
     _rows(x, "x", plan.tokens)
-    xs = torch.empty(plan.tokens * plan.top, x.shape[1], dtype=x.dtype, device=dev)
-    with _Queue(dev) as st:
-        _check(load_lm().nsparse_lm_gather_tokens(_DTYPES[x.dtype], _ptr(x), _ptr(plan.place), plan.tokens, plan.top, x.shape[1], _ptr(xs), st))
+    xs = torch.empty(plan.tokens * plan.top, x.shape[1], dtype=x.dtype, device=x.device)
+    _check(_queued(dev, load_lm().nsparse_lm_gather_tokens, _DTYPES[x.dtype], x.data_ptr(), plan.place.data_ptr(), plan.tokens, plan.top,
+                   x.shape[1], xs.data_ptr()))
     return xs
 
 
@@ -339,10 +341,9 @@ def _combine(y, plan, weights):
     dev = _on_gpu(y, plan.place, *([weights] if weights is not None else []))
     _rows(y, "y", plan.tokens * plan.top)
     _weights(weights, plan)
-    out = torch.empty(plan.tokens, y.shape[1], dtype=y.dtype, device=dev)
-    with _Queue(dev) as st:
-        _check(load_lm().nsparse_lm_combine_tokens(_DTYPES[y.dtype], _ptr(y), _ptr(plan.place), _ptr(weights), plan.tokens, plan.top, y.shape[1],
-                                                   _ptr(out), st))
+    out = torch.empty(plan.tokens, y.shape[1], dtype=y.dtype, device=y.device)
+    _check(_queued(dev, load_lm().nsparse_lm_combine_tokens, _DTYPES[y.dtype], y.data_ptr(), plan.place.data_ptr(), _ptr(weights), plan.tokens,
+                   plan.top, y.shape[1], out.data_ptr()))
     return out
 
 
@@ -401,9 +402,8 @@ def _combine_backward(dout, y, plan, weights, fill):
     _weights(weights, plan)
     dy = (torch.zeros_like if fill else torch.empty_like)(y)
     dw = torch.empty_like(weights)
-    with _Queue(dev) as st:
-        _check(load_lm().nsparse_lm_combine_tokens_bwd(_DTYPES[y.dtype], _ptr(dout), _ptr(y), _ptr(plan.place), _ptr(weights), plan.tokens,
-                                                       plan.top, y.shape[1], _ptr(dy), _ptr(dw), st))
+    _check(_queued(dev, load_lm().nsparse_lm_combine_tokens_bwd, _DTYPES[y.dtype], dout.data_ptr(), y.data_ptr(), plan.place.data_ptr(),
+                   weights.data_ptr(), plan.tokens, plan.top, y.shape[1], dy.data_ptr(), dw.data_ptr()))
     return dy, dw
 
 
