@@ -60,16 +60,43 @@ __global__ void __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256)
                 x[y] = group_of_chunk(G, c, u + y, shift, g);
                 whole = whole && x[y].rows == 16;
             }
+            // with few rows nobody else hides the way to memory: everything is asked for at once
+            constexpr bool kEarly = WAVES > 1 && DP * sizeof(T) <= 512;
+            Rows<T, E> ve[kEarly ? NG / 2 : 1];
+            auto load_v = [&](Rows<T, E> &vr, int y) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const Group16 &gx = x[y + (e >> 2)];
+                    const int r = 4 * quad + (e & 3);
+                    const T *p = v + gx.v_off + (long long)(r < gx.rows ? r : 0) * G.v_row + col * E;
+                    if constexpr (FULL) rows_load(vr, e, p); else rows_load_part(vr, e, p, D - col * E);
+                }
+            };
             // S^T, sixteen keys at a time
             f32x4 s[NG];
+            if constexpr (kEarly) {
+                Frag<T> kf[NG][KS];
 #pragma unroll
-            for (int y = 0; y < NG; y++) {
-                const int r = col < x[y].rows ? col : 0;
-                Frag<T> kf[KS];
-                row_frags<T, KS, FULL>(kf, k + x[y].k_off + (long long)r * G.k_row, quad, D, true);
-                s[y] = f32x4{0, 0, 0, 0};
+                for (int y = 0; y < NG; y++)
+                    row_frags<T, KS, FULL>(kf[y], k + x[y].k_off + (long long)(col < x[y].rows ? col : 0) * G.k_row, quad, D, true);
 #pragma unroll
-                for (int z = 0; z < KS; z++) s[y] = mma(kf[z], qf[z], s[y]);
+                for (int y = 0; y < NG; y += 2) load_v(ve[y / 2], y);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int y = 0; y < NG; y++) {
+                    s[y] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int z = 0; z < KS; z++) s[y] = mma(kf[y][z], qf[z], s[y]);
+                }
+            } else {
+#pragma unroll
+                for (int y = 0; y < NG; y++) {
+                    Frag<T> kf[KS];
+                    row_frags<T, KS, FULL>(kf, k + x[y].k_off + (long long)(col < x[y].rows ? col : 0) * G.k_row, quad, D, true);
+                    s[y] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int z = 0; z < KS; z++) s[y] = mma(kf[z], qf[z], s[y]);
+                }
             }
             float top = -INFINITY;
 #pragma unroll
@@ -99,15 +126,14 @@ __global__ void __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256)
             // O^T += V^T P^T, 32 keys at a time
 #pragma unroll
             for (int y = 0; y < NG; y += 2) {
-                Rows<T, E> vr;
+                Rows<T, E> late;
+                if constexpr (!kEarly) load_v(late, y);
+                Rows<T, E> &vr = kEarly ? ve[y / 2] : late;
+                // a hidden key's row must not reach the sum, whatever stands there
+                if (!whole) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const Group16 &gx = x[y + (e >> 2)];
-                    const int r = 4 * quad + (e & 3);
-                    const T *p = v + gx.v_off + (long long)(r < gx.rows ? r : 0) * G.v_row + col * E;
-                    if constexpr (FULL) rows_load(vr, e, p); else rows_load_part(vr, e, p, D - col * E);
-                    // a hidden key's row must not reach the sum, whatever stands there
-                    if (!whole && r >= gx.rows) rows_clear(vr, e);
+                    for (int e = 0; e < 8; e++)
+                        if (4 * quad + (e & 3) >= x[y + (e >> 2)].rows) rows_clear(vr, e);
                 }
                 const Frag<T> pf = frag_pack<T>(s[y], s[y + 1]);
 #pragma unroll

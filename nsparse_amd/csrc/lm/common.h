@@ -242,6 +242,16 @@ __device__ inline unsigned long long uniform64(unsigned long long v)
 {
     return ((unsigned long long)(unsigned)uniform((int)(v >> 32)) << 32) | (unsigned)uniform((int)v);
 }
+// over the wavefront, the result everywhere: inside the rows of sixteen by their neighbours, then over the four rows
+__device__ inline float wave_max(float x)
+{
+    x = fmaxf(x, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0xb1, 0xf, 0xf, false)));
+    x = fmaxf(x, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x4e, 0xf, 0xf, false)));
+    x = fmaxf(x, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x141, 0xf, 0xf, false)));
+    x = fmaxf(x, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x140, 0xf, 0xf, false)));
+    return quads_max(x);
+}
+
 // 2^x in one instruction; what is below 2^-126 becomes 0, which no sum next to a 1 can tell
 __device__ inline float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 

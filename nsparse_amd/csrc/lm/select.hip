@@ -209,7 +209,8 @@ __device__ inline unsigned order_key(float x)
 __device__ inline float key_value(unsigned k) { return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k); }
 
 // One wavefront: the best c.need of score[c.lo .. c.hi) (LDS, finite), each off by at most `off`; false: take the plain way.
-template <class T>
+// NV > 0: at most 64 NV scores, which stay in registers.
+template <class T, int NV>
 __device__ bool select_wave(const Geometry &G, const Seq &sq, int t, int g, const Competition &c, const T *q, const T *means, float off,
                             float *score, int *row)
 {
@@ -217,50 +218,56 @@ __device__ bool select_wave(const Geometry &G, const Seq &sq, int t, int g, cons
     // 2 off, rounded up through the additions below
     const float band = 2.0f * off;
     if (!(band < 1e30f)) return false;
-    float lo = INFINITY, hi = -INFINITY;
-    for (int x = c.lo + lane; x < c.hi; x += 64) {
-        const float s = score[x];
-        lo = fminf(lo, s);
-        hi = fmaxf(hi, s);
-    }
+    const int n = c.hi - c.lo;
+    float kept[NV > 0 ? NV : 1];
+    if constexpr (NV > 0) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        lo = fminf(lo, __shfl_xor(lo, d));
-        hi = fmaxf(hi, __shfl_xor(hi, d));
+        for (int v = 0; v < NV; v++) kept[v] = 64 * v + lane < n ? score[c.lo + 64 * v + lane] : -INFINITY;
     }
+    // f(score, its place) for 64 scores at a time; the places behind the last hold -inf
+    auto each = [&](auto f) {
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int v = 0; v < NV; v++)
+                if (64 * v < n) f(kept[v], 64 * v + lane);
+        } else {
+            for (int x = lane; x - lane < n; x += 64) f(x < n ? score[c.lo + x] : -INFINITY, x);
+        }
+    };
+    float lo = INFINITY, hi = -INFINITY;
+    each([&](float s, int x) {
+        lo = fminf(lo, x < n ? s : INFINITY);
+        hi = fmaxf(hi, s);
+    });
+    lo = -wave_max(-lo);
+    hi = wave_max(hi);
     // count(>= key_lo) >= need, count(>= key_hi) < need; by value while that halves well, then by the numbers' bits
-    unsigned key_lo = order_key(lo), key_hi = order_key(hi) + 1;
-    float a = lo;
+    unsigned key_lo = (unsigned)uniform((int)order_key(lo)), key_hi = (unsigned)uniform((int)order_key(hi)) + 1;
     for (int step = 0; key_hi - key_lo > 1; step++) {
         unsigned key = key_lo + (key_hi - key_lo) / 2;
         if (step < 14) {
             const float mid = 0.5f * key_value(key_lo) + 0.5f * key_value(key_hi - 1);
-            const unsigned k = order_key(mid);
+            const unsigned k = (unsigned)uniform((int)order_key(mid));
             if (k > key_lo && k < key_hi) key = k;
         }
         const float mid = key_value(key);
-        int n = 0;
-        for (int x = c.lo; x < c.hi; x += 64) n += __popcll(__ballot(x + lane < c.hi && score[x + lane] >= mid));
-        if (n >= c.need) key_lo = key; else key_hi = key;
-        if (n == c.need) break;
+        int m = 0;
+        each([&](float s, int) { m += __popcll(__ballot(s >= mid)); });
+        if (m >= c.need) key_lo = key; else key_hi = key;
+        if (m == c.need) break;
     }
-    {
-        // a: the need-th best
-        const float at_least = key_value(key_lo);
-        a = INFINITY;
-        for (int x = c.lo + lane; x < c.hi; x += 64)
-            if (score[x] >= at_least) a = fminf(a, score[x]);
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) a = fminf(a, __shfl_xor(a, d));
-    }
+    // a: the need-th best
+    const float at_least = key_value(key_lo);
+    float a = INFINITY;
+    each([&](float s, int) { a = s >= at_least ? fminf(a, s) : a; });
+    a = -wave_max(-a);
     const float slack = band + 4.0f * 5.9604645e-8f * (fabsf(a) + band);
     const float above = a + slack, below = a - slack;
     int sure = 0, between = 0;
-    for (int x = c.lo; x < c.hi; x += 64) {
-        const float s = x + lane < c.hi ? score[x + lane] : -INFINITY;
+    each([&](float s, int) {
         sure += __popcll(__ballot(s > above));
         between += __popcll(__ballot(s >= below && s <= above));
-    }
+    });
     const int places = c.need - sure;
     if (between != places) {
         if (between > 64) return false;
@@ -303,14 +310,18 @@ __device__ bool select_wave(const Geometry &G, const Seq &sq, int t, int g, cons
         if (eb >= 0) score[eb] = better < places ? INFINITY : -INFINITY;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int v = 0; v < NV; v++) kept[v] = 64 * v + lane < n ? score[c.lo + 64 * v + lane] : -INFINITY;
+        }
     }
     int at = c.lo;
-    for (int x = c.lo; x < c.hi; x += 64) {
-        const bool in = x + lane < c.hi && score[x + lane] >= below;
+    each([&](float s, int x) {
+        const bool in = s >= below;
         const unsigned long long m = __ballot(in);
-        if (in) row[at + __popcll(m & ((1ULL << lane) - 1))] = x + lane;
+        if (in) row[at + __popcll(m & ((1ULL << lane) - 1))] = c.lo + x;
         at += __popcll(m);
-    }
+    });
     return true;
 }
 
@@ -422,7 +433,8 @@ __global__ void __launch_bounds__(256)
             const Competition c = competition(G, sq, (int)(t - sq.q_base), first, local);
             int *row = idx + ((long long)t * G.kv_heads + g) * G.width;
             if (!write_forced(G, c, first, local, row, lane, 64)) continue;
-            if (!select_wave(G, sq, t, g, c, q, means, score_off(G, q_norm2[t - t0], m2), score + (t - t0) * LS, row)) plain_row[t - t0] = 1;
+            if (!select_wave<T, CAP <= 768 ? CAP / 64 : 0>(G, sq, t, g, c, q, means, score_off(G, q_norm2[t - t0], m2), score + (t - t0) * LS, row))
+                plain_row[t - t0] = 1;
         }
         __syncthreads();
         for (int t = a; t < z; t++)
@@ -474,28 +486,44 @@ __global__ void __launch_bounds__(1024)
 #pragma unroll
     for (int d = 1; d < 16; d <<= 1) q2 += __shfl_xor(q2, d);
     float n2max = 0.f;
-    for (int b = c.lo + (int)(threadIdx.x >> 4); b < c.hi; b += 64) {
-        const T *p = mean_of_block(G, sq, means, g, b);
-        float dot = 0.f, n2 = 0.f;
+    // four blocks at a time: their pages are all asked for, then their means, before any is used
+    for (int b0 = c.lo + (int)(threadIdx.x >> 4); b0 < c.hi; b0 += 256) {
+        const T *p[4];
+        T8 x[4][2];
 #pragma unroll
-        for (int z = 0; z < 2; z++) {
-            const int d = 128 * z + 8 * l16;
-            if (p && d < G.head_dim) {
-                const T8 x = __builtin_bit_cast(T8, frag_load(p + d));
+        for (int u = 0; u < 4; u++) {
+            const int b = b0 + 64 * u;
+            p[u] = b < c.hi ? mean_of_block(G, sq, means, g, b) : nullptr;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int z = 0; z < 2; z++) {
+                const int d = 128 * z + 8 * l16;
+                x[u][z] = T8{};
+                if (p[u] && d < G.head_dim) x[u][z] = __builtin_bit_cast(T8, frag_load(p[u] + d));
+            }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int b = b0 + 64 * u;
+            float dot = 0.f, n2 = 0.f;
+#pragma unroll
+            for (int z = 0; z < 2; z++)
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    dot += s[8 * z + e] * (float)x[e];
-                    n2 += (float)x[e] * (float)x[e];
+                    dot += s[8 * z + e] * (float)x[u][z][e];
+                    n2 += (float)x[u][z][e] * (float)x[u][z][e];
                 }
+#pragma unroll
+            for (int d = 1; d < 16; d <<= 1) {
+                dot += __shfl_xor(dot, d);
+                n2 += __shfl_xor(n2, d);
+            }
+            if (b < c.hi) {
+                n2max = max_or_nan(n2max, p[u] ? n2 : NAN);
+                if (l16 == 0) score[b] = dot;
             }
         }
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) {
-            dot += __shfl_xor(dot, d);
-            n2 += __shfl_xor(n2, d);
-        }
-        n2max = max_or_nan(n2max, p ? n2 : NAN);
-        if (l16 == 0) score[b] = dot;
     }
 #pragma unroll
     for (int d = 16; d < 64; d <<= 1) n2max = max_or_nan(n2max, __shfl_xor(n2max, d));
@@ -504,7 +532,7 @@ __global__ void __launch_bounds__(1024)
     if (wave == 0) {
         float m2 = norms[0];
         for (int w = 1; w < 16; w++) m2 = max_or_nan(m2, norms[w]);
-        const bool done = select_wave(G, sq, t, g, c, q, means, score_off(G, q2, m2), score, row);
+        const bool done = select_wave<T, 0>(G, sq, t, g, c, q, means, score_off(G, q2, m2), score, row);
         if (lane == 0) plain = !done;
     }
     __syncthreads();
