@@ -243,7 +243,8 @@ __device__ bool select_wave(const Geometry &G, const Seq &sq, int t, int g, cons
     hi = wave_max(hi);
     // count(>= key_lo) >= need, count(>= key_hi) < need; by value while that halves well, then by the numbers' bits
     unsigned key_lo = (unsigned)uniform((int)order_key(lo)), key_hi = (unsigned)uniform((int)order_key(hi)) + 1;
-    for (int step = 0; key_hi - key_lo > 1; step++) {
+    int m_lo = n;
+    for (int step = 0; key_hi - key_lo > 1 && m_lo != c.need; step++) {
         unsigned key = key_lo + (key_hi - key_lo) / 2;
         if (step < 14) {
             const float mid = 0.5f * key_value(key_lo) + 0.5f * key_value(key_hi - 1);
@@ -253,8 +254,12 @@ __device__ bool select_wave(const Geometry &G, const Seq &sq, int t, int g, cons
         const float mid = key_value(key);
         int m = 0;
         each([&](float s, int) { m += __popcll(__ballot(s >= mid)); });
-        if (m >= c.need) key_lo = key; else key_hi = key;
-        if (m == c.need) break;
+        if (m >= c.need) {
+            key_lo = key;
+            m_lo = m;
+        } else {
+            key_hi = key;
+        }
     }
     // a: the need-th best
     const float at_least = key_value(key_lo);
@@ -348,8 +353,9 @@ __global__ void __launch_bounds__(256)
     __shared__ Plain pl;
     const int lane = lane_id(), col = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int g = (int)(blockIdx.x % G.kv_heads);
-    const int t0 = (int)(blockIdx.x / G.kv_heads) * 16;
+    const int g = (int)((gridDim.x - 1 - blockIdx.x) % G.kv_heads);
+    // the last rows, which see most, begin first
+    const int t0 = (int)((gridDim.x - 1 - blockIdx.x) / G.kv_heads) * 16;
     const int t1 = t0 + 16 < G.q_rows ? t0 + 16 : G.q_rows;
     if (threadIdx.x < 16) plain_row[threadIdx.x] = 0;
     // the group's summed queries, and the norm of the sum of their absolute values
@@ -532,7 +538,9 @@ __global__ void __launch_bounds__(1024)
     if (wave == 0) {
         float m2 = norms[0];
         for (int w = 1; w < 16; w++) m2 = max_or_nan(m2, norms[w]);
-        const bool done = select_wave<T, 0>(G, sq, t, g, c, q, means, score_off(G, q2, m2), score, row);
+        const float off = score_off(G, q2, m2);
+        const bool done = c.hi - c.lo <= 512 ? select_wave<T, 8>(G, sq, t, g, c, q, means, off, score, row)
+                                             : select_wave<T, 0>(G, sq, t, g, c, q, means, off, score, row);
         if (lane == 0) plain = !done;
     }
     __syncthreads();
