@@ -19,27 +19,29 @@ namespace lm {
 // delta comes from the output as the forward rounded it.  That rounding matters where few keys share the weight, so workgroups with
 // at most kExact keys in their union walk twice and take delta = sum p (dout . v) from the first walk.  In single precision the
 // probabilities are divided by their sum, which takes the rounding of the log-sum-exp out of them.
+// 32 keys a step and one set of columns a wavefront leave three wavefronts a SIMD, which hide each other's reads of LDS, its
+// bound.  4096 rows of 32 heads of 128, 16 blocks each, bf16, against two sets and 64 keys a step (as the forward has where blocks allow):
+// blocks of 64: 277 against 313 us, of 32: 195 against 318, of 16: 148 against 210.
 constexpr int kExact = 256;
 struct RowInfo {  // of a query row and head, for dk and dv
     float lse2, delta, inv;
     float pad;
 };
-template <class T, int DP, int NT, int NG, bool WIDE>
+template <class T, int DP, bool WIDE>
 __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
     k_attend_dq(const Geometry G, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ idx,
                 const T *__restrict__ out, const float *__restrict__ lse, const T *__restrict__ dout, T *__restrict__ dq,
                 RowInfo *__restrict__ info, int slices, int per_tile)
 {
-    constexpr int KS = DP / 32, E = DP / 16, kTile = NG * 16 * Tile<T, DP>::kPieces;
+    constexpr int KS = DP / 32, E = DP / 16, NG = 2 /* groups of sixteen keys a step */, kTile = NG * 16 * Tile<T, DP>::kPieces;
     __shared__ u32x4 kt[2][kTile], vt[2][kTile];
     __shared__ Union un;
     const int wave = uniform((int)(threadIdx.x >> 6));
     const int g = (int)(blockIdx.x % G.kv_heads);
     const int rest = (int)(blockIdx.x / G.kv_heads);
     const int slice = rest % slices;
-    const int per_wave = NT * per_tile;  // rows a wavefront
-    const int t0 = (rest / slices) * 4 * per_wave;
-    const int t1 = t0 + 4 * per_wave < G.q_rows ? t0 + 4 * per_wave : G.q_rows;
+    const int t0 = (rest / slices) * 4 * per_tile;
+    const int t1 = t0 + 4 * per_tile < G.q_rows ? t0 + 4 * per_tile : G.q_rows;
     const int D = G.head_dim;
     const float sl2 = G.scale * kLog2e;
 
@@ -53,42 +55,32 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
         const int z = sq.q_base + sq.q_len < t1 ? (int)(sq.q_base + sq.q_len) : t1;
         const Column c0(G, g, slice, per_tile);
         const int col = c0.col, quad = c0.quad;
-        // lane i's row for the walk; a column's row is number (wave * NT + x) * per_tile + Column::sub
+        // lane i's row for the walk; a column's row is number wave * per_tile + Column::sub
         const int t_mine = t0 + opaque(lane_id());
         const int limit = t_mine >= a && t_mine < z ? visible_keys(G, sq, (int)(t_mine - sq.q_base)) : 0;
-        Frag<T> qf[NT][KS], gf[NT][KS];
-        int lim[NT], num[NT];
-        float lse2[NT], rounded[NT];
+        Frag<T> qf[KS], gf[KS];
+        const int num = wave * per_tile + c0.sub;
+        const bool on = c0.live && t0 + num >= a && t0 + num < z;
+        int lim = pull(limit, num);
+        if (!on) lim = 0;
+        const int t = on ? t0 + num : a;
+        const long long th = (long long)t * G.heads + c0.head;
+        row_frags<T, KS, false>(gf, dout + th * D, quad, D, on);
+        row_frags<T, KS, false>(qf, out + th * D, quad, D, on);
+        float rounded = 0.f;
 #pragma unroll
-        for (int x = 0; x < NT; x++) {
-            num[x] = (wave * NT + x) * per_tile + c0.sub;
-            const bool on = c0.live && t0 + num[x] >= a && t0 + num[x] < z;
-            lim[x] = pull(limit, num[x]);
-            if (!on) lim[x] = 0;
-            const int t = on ? t0 + num[x] : a;
-            const long long th = (long long)t * G.heads + c0.head;
-            row_frags<T, KS, false>(gf[x], dout + th * D, quad, D, on);
-            row_frags<T, KS, false>(qf[x], out + th * D, quad, D, on);
-            rounded[x] = 0.f;
-#pragma unroll
-            for (int w = 0; w < KS; w++) rounded[x] += frag_dot(gf[x][w], qf[x][w]);
-            rounded[x] = quads_sum(rounded[x]);
-            row_frags<T, KS, false>(qf[x], q + (long long)t * G.q_row + (long long)c0.head * G.q_head, quad, D, on);
-            lse2[x] = on ? lse[th] * kLog2e : INFINITY;
-        }
+        for (int w = 0; w < KS; w++) rounded += frag_dot(gf[w], qf[w]);
+        rounded = quads_sum(rounded);
+        row_frags<T, KS, false>(qf, q + (long long)t * G.q_row + (long long)c0.head * G.q_head, quad, D, on);
+        const float lse2 = on ? lse[th] * kLog2e : INFINITY;
         const int count = z - a;
         const unsigned long long every = (count < 64 ? (1ULL << count) - 1 : ~0ULL) << (a - t0);
         unsigned long long todo = every, now = every;
         while (todo) {
-            f32x4 o[NT][E];
-            float total[NT], with_dp[NT], delta[NT];
+            f32x4 o[E];
+            float total = 0.f, with_dp = 0.f, delta = rounded;
 #pragma unroll
-            for (int x = 0; x < NT; x++) {
-                total[x] = with_dp[x] = 0.f;
-                delta[x] = rounded[x];
-#pragma unroll
-                for (int j = 0; j < E; j++) o[x][j] = f32x4{0, 0, 0, 0};
-            }
+            for (int j = 0; j < E; j++) o[j] = f32x4{0, 0, 0, 0};
             const int blocks = (read_lane(limit, 63 - __builtin_clzll(now)) + G.block - 1) / G.block;
             for (int b0 = 0; b0 < blocks; b0 += kRange) {
                 union_build(un, G, idx, g, t0, now, limit, b0, blocks - b0 < kRange ? blocks - b0 : kRange, wave);
@@ -109,58 +101,37 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
                             tile_load<T, DP, NG, WIDE>(kt[buf ^ 1], k, next.k_off, next, G.k_row, D);
                             tile_load<T, DP, NG, WIDE>(vt[buf ^ 1], v, next.v_off, next, G.v_row, D);
                         }
-                        const bool use = (st.any >> (wave * NT * per_tile)) & (NT * per_tile < 64 ? (1ULL << (NT * per_tile)) - 1 : ~0ULL);
+                        const bool use = (st.any >> (wave * per_tile)) & ((1ULL << per_tile) - 1);
                         if (use) {
+                            f32x4 s[2], d[2];
+                            s[0] = s[1] = d[0] = d[1] = f32x4{0, 0, 0, 0};
+                            pipelined<Frag<T>, 4 * KS, 4, 2>(
+                                [&](int i) { return tile_frag<T, DP>(i < 2 * KS ? kt[buf] : vt[buf], 16 * (i / KS & 1) + col, i % KS, quad); },
+                                [&](int i, const Frag<T> &f) {
+                                    const int y = i / KS & 1;
+                                    if (i < 2 * KS) s[y] = mma(f, qf[i % KS], s[y]);
+                                    else d[y] = mma(f, gf[i % KS], d[y]);
+                                });
 #pragma unroll
-                            for (int y2 = 0; y2 < NG; y2 += 2) {
-                                Frag<T> pf[NT];
-                                f32x4 s[NT][2], d[NT][2];
+                            for (int y = 0; y < 2; y++) {
+                                const int vis = (st.lists(y) >> num) & 1 ? lim - st.first(y) - 4 * quad : 0;
 #pragma unroll
-                                for (int x = 0; x < NT; x++) s[x][0] = s[x][1] = d[x][0] = d[x][1] = f32x4{0, 0, 0, 0};
-                                pipelined<Frag<T>, 4 * KS, 4, 2>(
-                                    [&](int i) {
-                                        const int r = 16 * (y2 + (i / KS & 1)) + col;
-                                        return tile_frag<T, DP>(i < 2 * KS ? kt[buf] : vt[buf], r, i % KS, quad);
-                                    },
-                                    [&](int i, const Frag<T> &f) {
-                                        const int y = i / KS & 1;
-#pragma unroll
-                                        for (int x = 0; x < NT; x++) {
-                                            if (i < 2 * KS) s[x][y] = mma(f, qf[x][i % KS], s[x][y]);
-                                            else d[x][y] = mma(f, gf[x][i % KS], d[x][y]);
-                                        }
-                                    });
-#pragma unroll
-                                for (int x = 0; x < NT; x++) {
-#pragma unroll
-                                    for (int y = 0; y < 2; y++) {
-                                        const bool on = (st.lists(y2 + y) >> num[x]) & 1;
-                                        const int vis = on ? lim[x] - st.first(y2 + y) - 4 * quad : 0;
-#pragma unroll
-                                        for (int e = 0; e < 4; e++) {
-                                            const float p = e < vis ? pow2(__builtin_fmaf(s[x][y][e], sl2, -lse2[x])) : 0.f;
-                                            if (pass == 0) with_dp[x] += p * d[x][y][e];
-                                            if (pass == 0 || sizeof(T) == 4) total[x] += p;
-                                            s[x][y][e] = p * (d[x][y][e] - delta[x]) * G.scale;
-                                        }
-                                    }
-                                    pf[x] = frag_pack<T>(s[x][0], s[x][1]);
+                                for (int e = 0; e < 4; e++) {
+                                    const float p = e < vis ? pow2(__builtin_fmaf(s[y][e], sl2, -lse2)) : 0.f;
+                                    if (pass == 0) with_dp += p * d[y][e];
+                                    if (pass == 0 || sizeof(T) == 4) total += p;
+                                    s[y][e] = p * (d[y][e] - delta) * G.scale;
                                 }
-                                if (pass == 0) continue;
+                            }
+                            if (pass == 1) {
+                                const Frag<T> pf = frag_pack<T>(s[0], s[1]);
+                                const Columns<T, DP> c(kt[buf], 0, quad, col);
                                 if constexpr (sizeof(T) == 2) {
-                                    pipelined<Frag<T>, E, 4, 2>([&](int i) { return Columns<T, DP>(kt[buf], y2, quad, col).frag(i); },
-                                                                [&](int i, const Frag<T> &f) {
-#pragma unroll
-                                                                    for (int x = 0; x < NT; x++) o[x][i] = mma(f, pf[x], o[x][i]);
-                                                                });
+                                    pipelined<Frag<T>, E, 4, 2>([&](int i) { return c.frag(i); },
+                                                                [&](int i, const Frag<T> &f) { o[i] = mma(f, pf, o[i]); });
                                 } else {
-                                    const Columns<T, DP> c(kt[buf], y2, quad, col);
 #pragma unroll
-                                    for (int j = 0; j < E; j++) {
-                                        const Frag<T> f = c.frag(j);
-#pragma unroll
-                                        for (int x = 0; x < NT; x++) o[x][j] = mma(f, pf[x], o[x][j]);
-                                    }
+                                    for (int j = 0; j < E; j++) o[j] = mma(c.frag(j), pf, o[j]);
                                 }
                             }
                         }
@@ -168,41 +139,31 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
                         __syncthreads();
                     }
                     if (pass == 0) {
-#pragma unroll
-                        for (int x = 0; x < NT; x++) {
-                            const float w = quads_sum(with_dp[x]), l = quads_sum(total[x]);
-                            delta[x] = l > 0.f ? w / l : 0.f;
-                            total[x] = 0.f;
-                        }
+                        const float w = quads_sum(with_dp), l = quads_sum(total);
+                        delta = l > 0.f ? w / l : 0.f;
+                        total = 0.f;
                     }
                 }
             }
             // A value that is no number reaches the columns that do not see it as 0 x NaN: then every row by itself.
-            bool bad = false;
+            float sum = delta;
 #pragma unroll
-            for (int x = 0; x < NT; x++) {
-                float t = delta[x];
-#pragma unroll
-                for (int j = 0; j < E; j++) t += (o[x][j][0] + o[x][j][1]) + (o[x][j][2] + o[x][j][3]);
-                bad = bad || !(fabsf(t) < INFINITY);
-            }
-            if ((now & (now - 1)) && __syncthreads_or(bad)) {
+            for (int j = 0; j < E; j++) sum += (o[j][0] + o[j][1]) + (o[j][2] + o[j][3]);
+            if ((now & (now - 1)) && __syncthreads_or(!(fabsf(sum) < INFINITY))) {
                 now = todo & -todo;
                 continue;
             }
             const Column c1(G, g, slice, per_tile);
-#pragma unroll
-            for (int x = 0; x < NT; x++) {
-                float inv = 1.f;
-                if (sizeof(T) == 4) {
-                    const float l = quads_sum(total[x]);
-                    inv = l > 0.f ? 1.f / l : 1.f;
-                }
-                const int n = (wave * NT + x) * per_tile + c1.sub;
-                if (!c1.live || !((now >> n) & 1)) continue;
-                const long long th = (long long)(t0 + n) * G.heads + c1.head;
-                store_row<T, DP>(dq + th * D, o[x], inv, c1.quad, D);
-                if (c1.quad == 0) info[th] = RowInfo{lse2[x], delta[x], inv, 0.f};
+            float inv = 1.f;
+            if (sizeof(T) == 4) {
+                const float l = quads_sum(total);
+                inv = l > 0.f ? 1.f / l : 1.f;
+            }
+            const int n = wave * per_tile + c1.sub;
+            if (c1.live && ((now >> n) & 1)) {
+                const long long at = (long long)(t0 + n) * G.heads + c1.head;
+                store_row<T, DP>(dq + at * D, o, inv, c1.quad, D);
+                if (c1.quad == 0) info[at] = RowInfo{lse2, delta, inv, 0.f};
             }
             todo &= ~now;
             now = todo & -todo;
@@ -323,9 +284,7 @@ __global__ void __launch_bounds__(1024)
 // products, and ROWS of them one behind the other, each with its own 32 of the (query, head) pairs that list the block.
 // The pairs' rows of q and dout go through LDS (by rows for S = Q K^T and dP = dO V^T, transposed for dK^T = Q^T dS and
 // dV^T = dO^T P), fetched while the 32 before are computed.  Bound by what LDS delivers: the more keys a wavefront, the fewer reads a product.
-#ifndef NSP_ITEMS
-#define NSP_ITEMS 1024
-#endif
+constexpr int kItems = 1024;
 constexpr int kListed = 1024;
 template <class T, int DP, int KW, int KEYS, int ROWS> struct Dkv {
     static constexpr int KS = DP / 32, E = DP / 16, kThreads = 64 * KEYS * ROWS, kStep = 32 * ROWS;
@@ -670,7 +629,7 @@ static BwdSpace bwd_space(const Geometry &G)
     // about 1024 items besides the blocks' own, of at least 64 rows
     const long long listed = (long long)G.q_rows * G.kv_heads * G.width;
     s.per_item = 64;
-    while (listed / s.per_item > NSP_ITEMS) s.per_item *= 2;
+    while (listed / s.per_item > kItems) s.per_item *= 2;
     s.shared_out = G.q_rows > s.per_item;
     s.max_items = s.gms + (s.shared_out ? listed / s.per_item : 0);
     // a block with n > per_item rows has at most 2 n / per_item items
@@ -704,7 +663,7 @@ static void launch_dkv(const Geometry &G, const void *q, const void *k, const vo
                            slots, (T *)dk, (T *)dv, sp.parts);
 }
 
-template <class T, int DP, int NG>
+template <class T, int DP>
 static void launch_bwd(const Geometry &G, const void *q, const void *k, const void *v, const int *idx, const void *out, const float *lse,
                        const void *dout, void *dq, void *dk, void *dv, char *ws, const BwdSpace &sp, hipStream_t st)
 {
@@ -713,20 +672,11 @@ static void launch_bwd(const Geometry &G, const void *q, const void *k, const vo
     const int slices = (int)ceil_div(G.group, 16);
     if (G.q_rows > 0) {
         const int per_tile = G.group < 16 ? 16 / G.group : 1;
-#define NSP_GO(NT, WIDE)                                                                                                                     \
-    hipLaunchKernelGGL((k_attend_dq<T, DP, NT, NG, WIDE>), dim3((unsigned)(ceil_div(G.q_rows, 4 * NT * per_tile) * slices * G.kv_heads)), \
+#define NSP_GO(WIDE)                                                                                                                     \
+    hipLaunchKernelGGL((k_attend_dq<T, DP, WIDE>), dim3((unsigned)(ceil_div(G.q_rows, 4 * per_tile) * slices * G.kv_heads)), \
                        dim3(256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx, (const T *)out, lse, (const T *)dout, (T *)dq,    \
                        info, slices, per_tile)
-        bool two = false;
-        if constexpr (sizeof(T) == 2 && DP <= 128) {
-            two = per_tile <= 8 && (long long)G.q_rows * slices * G.kv_heads >= 2 * per_tile * 2048LL;
-            if (two) {
-                if (G.block >= 16 * NG) NSP_GO(2, true); else NSP_GO(2, false);
-            }
-        }
-        if (!two) {
-            if (G.block >= 16 * NG) NSP_GO(1, true); else NSP_GO(1, false);
-        }
+        if (G.block >= 32) NSP_GO(true); else NSP_GO(false);
 #undef NSP_GO
         if (sp.gms > 0) {
             hipLaunchKernelGGL(k_pattern_bits, dim3((unsigned)((long long)sp.words * G.kv_heads)), dim3(256), 0, st, G, idx, bits, sp.words);
@@ -786,13 +736,13 @@ int nsparse_lm_block_attention_bwd(const nsparse_lm_attn *a, const void *q, cons
         return fail(NSPARSE_LM_EWORKSPACE, "block_attention_bwd: workspace smaller than nsparse_lm_block_attention_bwd_workspace() says");
     hipStream_t st = (hipStream_t)stream;
     char *ws = (char *)workspace;
-#define NSP_DIM(T, NG)                                                                                                  \
-    if (G.head_dim <= 64) launch_bwd<T, 64, NG>(G, q, k, v, idx, out, lse, dout, dq, dk, dv, ws, sp, st);               \
-    else if (G.head_dim <= 128) launch_bwd<T, 128, NG>(G, q, k, v, idx, out, lse, dout, dq, dk, dv, ws, sp, st);        \
-    else launch_bwd<T, 256, 2>(G, q, k, v, idx, out, lse, dout, dq, dk, dv, ws, sp, st)
-    if (a->dtype == NSPARSE_LM_BF16) { NSP_DIM(__bf16, 4); }
-    else if (a->dtype == NSPARSE_LM_F16) { NSP_DIM(_Float16, 4); }
-    else { NSP_DIM(float, 2); }
+#define NSP_DIM(T)                                                                                                  \
+    if (G.head_dim <= 64) launch_bwd<T, 64>(G, q, k, v, idx, out, lse, dout, dq, dk, dv, ws, sp, st);               \
+    else if (G.head_dim <= 128) launch_bwd<T, 128>(G, q, k, v, idx, out, lse, dout, dq, dk, dv, ws, sp, st);        \
+    else launch_bwd<T, 256>(G, q, k, v, idx, out, lse, dout, dq, dk, dv, ws, sp, st)
+    if (a->dtype == NSPARSE_LM_BF16) { NSP_DIM(__bf16); }
+    else if (a->dtype == NSPARSE_LM_F16) { NSP_DIM(_Float16); }
+    else { NSP_DIM(float); }
 #undef NSP_DIM
     return launched("block_attention_bwd");
 }

@@ -391,10 +391,10 @@ static void launch_tiles(const Geometry &G, const void *q, const void *k, const 
     const int slices = (int)ceil_div(G.group, 16);
     const int per_tile = G.group < 16 ? 16 / G.group : 1;
     const dim3 grid((unsigned)(ceil_div(G.q_rows, 4 * NT * per_tile) * slices * G.kv_heads));
-    if (G.block >= 16 * NG)
+    if (NG == 4 || G.block >= 16 * NG)
         hipLaunchKernelGGL((k_attend_tiles<T, DP, NT, NG, true>), grid, dim3(256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx,
                            (T *)out, lse, slices, per_tile);
-    else
+    else if constexpr (NG == 2)
         hipLaunchKernelGGL((k_attend_tiles<T, DP, NT, NG, false>), grid, dim3(256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx,
                            (T *)out, lse, slices, per_tile);
 }
