@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256)
                 whole = whole && x[y].rows == 16;
             }
             // with few rows nobody else hides the way to memory: everything is asked for at once
-            constexpr bool kEarly = WAVES > 1 && DP * sizeof(T) <= 512;
+            constexpr bool kEarly = WAVES > 1;
             Rows<T, E> ve[kEarly ? NG / 2 : 1];
             auto load_v = [&](Rows<T, E> &vr, int y) {
 #pragma unroll
@@ -404,9 +404,12 @@ static void launch_attend(const Geometry &G, const void *q, const void *k, const
 {
     const int slices = (int)ceil_div(G.group, 16);
     const long long rows = (long long)G.q_rows * slices;
-    // eight wavefronts a row while that leaves compute units without work otherwise
+    // several wavefronts a row while that leaves compute units without work otherwise (8 key heads, 16 blocks of 64: 64 sequences 47
+    // against 83 us, 128: 107 and 108; 4 key heads, 8 blocks of 32: 512 sequences 31.5 against 25.6)
     const bool split = rows * G.kv_heads < 2048;
     const bool full = G.head_dim == DP;
+    // neighbouring rows together where there are some (256 sequences of 3 new tokens: 357 against 297 us row by row, of 4: 224;
+    // but 512 of 2, 2 heads each and blocks of 16: 57 against 200)
     if (!split && G.q_rows / G.n_seq >= 4) {
         // 64 keys a step where a block has them, else 32 (blocks of 32 in steps of 64: 58 against 39 us for 3945 rows of 16 heads)
         const int per_tile = G.group < 16 ? 16 / G.group : 1;
@@ -424,7 +427,8 @@ static void launch_attend(const Geometry &G, const void *q, const void *k, const
     hipLaunchKernelGGL((k_attend<T, DP, NG, FULL, WAVES>), dim3((unsigned)((WAVES > 1 ? rows : ceil_div(G.q_rows, 4) * slices) * G.kv_heads)), \
                        dim3(WAVES > 1 ? 64 * WAVES : 256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx, (T *)out, lse, slices)
     if (split) {
-        if (full) NSP_GO(true, 8); else NSP_GO(false, 8);
+        constexpr int kSplit = DP * sizeof(T) > 512 ? 4 : 8;  // registers for a row's sums and a step's keys and values
+        if (full) NSP_GO(true, kSplit); else NSP_GO(false, kSplit);
     } else {
         if (full) NSP_GO(true, 1); else NSP_GO(false, 1);
     }
