@@ -66,7 +66,8 @@ const char *nsparse_lm_build_info(void);
  * Pattern.  idx int[q_rows, kv_heads, width]: the blocks (of `block` keys, numbered inside the sequence) that the query's
  * heads of group g attend to.  An entry counts only if it is not negative, lies inside the sequence and is greater
  * than every entry before it in its row; others are skipped (so -1 ends a row, and a block listed twice counts once).
- * A query with no key left gets out = 0 and lse = -inf, and gradients 0.
+ * A query with no key left gets out = 0 and lse = -inf, and gradients 0.  Whatever stands in keys and values that a query does not see
+ * (NaN included) does not reach its outputs; a query whose own q or dout is no number spoils dk and dv of the blocks that it lists.
  *
  * Block means.  One row [kv_heads, head_dim] a block, in the keys' type, contiguous.  The row of block b of sequence s:
  *   paged     page * (page_size / block) + block inside the page       k_rows * page_size / block rows
@@ -84,7 +85,7 @@ typedef struct nsparse_lm_attn {
     int page_size;              /* 0, or a multiple of block */
     int first, local;           /* selection: the first and the last eligible blocks always taken; see select_blocks */
     float scale;                /* of q.k in the softmax; finite */
-    long long q_rows, k_rows;
+    long long q_rows, k_rows;   /* a sequence has at most 2^31 - 4097 keys; q_rows x heads is limited alike */
     long long table_stride;     /* entries of page_table a sequence */
     const int *cu_q, *cu_k, *q_len, *k_len, *page_table;
     long long q_stride[2];      /* row, head */
@@ -120,7 +121,7 @@ int nsparse_lm_block_attention_bwd(const nsparse_lm_attn *a, const void *q, cons
  *   offsets int[experts + 1]   sorted rows [offsets[e], offsets[e+1]) belong to expert e
  *   order   int[tokens * top]  sorted row -> entry; rows behind offsets[experts] are left as they were
  *   place   int[tokens * top]  entry -> sorted row, -1 where dropped
- * tokens * top < 2^31 - 4096, experts <= 4096. */
+ * tokens * top < 2^31 - 4096, experts <= 4096, channels <= 2^28. */
 long long nsparse_lm_route_workspace(long long tokens, int top, int experts);
 int nsparse_lm_route(const int *ids, long long tokens, int top, int experts, int *offsets, int *order, int *place,
                      void *workspace, long long workspace_bytes, void *stream);

@@ -46,16 +46,17 @@ int geometry(const nsparse_lm_attn *a, bool needs_q, bool needs_k, Geometry *g)
     if (a->n_seq < 1) return fail(NSPARSE_LM_EARG, "n_seq must be positive");
     if (a->q_rows < 0 || a->q_rows > 0x7fffffffLL / 2 || a->k_rows < 0) return fail(NSPARSE_LM_EARG, "q_rows or k_rows out of range");
     // one workgroup index per (query row, key head, slice of 16 heads)
-    if (a->q_rows * (a->kv_heads + (long long)a->heads / 16) > 0x7fffffffLL) return fail(NSPARSE_LM_EARG, "q_rows x heads out of range");
+    if (a->q_rows * (a->kv_heads + (long long)a->heads / 16) > kMostGroups) return fail(NSPARSE_LM_EARG, "q_rows x heads out of range");
     if (a->page_size < 0 || a->page_size % a->block) return fail(NSPARSE_LM_EARG, "page_size must be a multiple of block");
     if (a->page_size > 0) {
         if (!a->k_len || !a->page_table) return fail(NSPARSE_LM_EARG, "a paged cache needs k_len and page_table");
         if (a->cu_k) return fail(NSPARSE_LM_EARG, "cu_k does not go with a paged cache");
+        if (a->k_rows > 0x7fffffffLL) return fail(NSPARSE_LM_EARG, "k_rows out of range");
         if (a->table_stride < 0 || a->table_stride > 0x7fffffffLL / a->page_size) return fail(NSPARSE_LM_EARG, "table_stride out of range");
     } else {
         if (a->page_table) return fail(NSPARSE_LM_EARG, "page_table without page_size");
         if (!a->cu_k && a->k_rows % a->n_seq) return fail(NSPARSE_LM_EARG, "k_rows must divide by n_seq where cu_k is absent");
-        if ((a->cu_k ? a->k_rows : a->k_rows / a->n_seq) > 0x7fffffffLL) return fail(NSPARSE_LM_EARG, "k_rows out of range");
+        if ((a->cu_k ? a->k_rows : a->k_rows / a->n_seq) > kMostKeys) return fail(NSPARSE_LM_EARG, "k_rows out of range");
     }
     if (!a->cu_q && a->q_rows % a->n_seq) return fail(NSPARSE_LM_EARG, "q_rows must divide by n_seq where cu_q is absent");
     const int per16 = 16 / elem_size(a->dtype);

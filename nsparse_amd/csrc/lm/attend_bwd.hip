@@ -37,8 +37,8 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
     __shared__ u32x4 kt[2][kTile], vt[2][kTile];
     __shared__ Union un;
     const int wave = uniform((int)(threadIdx.x >> 6));
-    const int g = (int)(blockIdx.x % G.kv_heads);
-    const int rest = (int)(blockIdx.x / G.kv_heads);
+    const int g = (int)(group_id() % G.kv_heads);
+    const int rest = (int)(group_id() / G.kv_heads);
     const int slice = rest % slices;
     const int t0 = (rest / slices) * 4 * per_tile;
     const int t1 = t0 + 4 * per_tile < G.q_rows ? t0 + 4 * per_tile : G.q_rows;
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(256)
     k_pattern_bits(const Geometry G, const int *__restrict__ idx, unsigned long long *__restrict__ bits, int words)
 {
     __shared__ Union un;
-    const int g = (int)(blockIdx.x % G.kv_heads), w = (int)(blockIdx.x / G.kv_heads);
+    const int g = (int)(group_id() % G.kv_heads), w = (int)(group_id() / G.kv_heads);
     const int wave = uniform((int)(threadIdx.x >> 6));
     const int t0 = w * 64, t1 = t0 + 64 < G.q_rows ? t0 + 64 : G.q_rows;
     for (int a = t0; a < t1;) {
@@ -222,7 +222,7 @@ struct Item {
 __global__ void __launch_bounds__(256)
     k_count_rows(const Geometry G, const unsigned long long *__restrict__ bits, int *__restrict__ counts, long long gms, int words)
 {
-    const long long gm = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long long gm = (long long)group_id() * 4 + (threadIdx.x >> 6);
     if (gm >= gms) return;
     Seq sq;
     int b, n = 0, w0, w1;
@@ -328,8 +328,8 @@ __global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>:
     const int wave = uniform(tid >> 6), kw = wave % KEYS, rw = wave / KEYS;
     const auto qt = [&](int buf) { return tiles + buf * C::kTile; };
     const auto gt = [&](int buf) { return tiles + (2 + buf) * C::kTile; };
-    const int part = (int)(blockIdx.x % parts);
-    Item it{(int)(blockIdx.x / parts), 0, 0x7fffffff, 0, 1, 0};
+    const int part = (int)(group_id() % parts);
+    Item it{(int)(group_id() / parts), 0, 0x7fffffff, 0, 1, 0};
     if (items) {
         if (it.gm >= *n_items) return;
         it = items[it.gm];
@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(64 * KEYS)
                T *__restrict__ dv, int parts)
 {
     using C = Dkv<T, DP, KW, KEYS, ROWS>;
-    const int part = (int)(blockIdx.x % parts), i = (int)(blockIdx.x / parts);
+    const int part = (int)(group_id() % parts), i = (int)(group_id() / parts);
     if (i >= *n_items) return;
     const Item it = items[i];
     if (it.chunks < 2 || it.chunk != 0) return;
@@ -655,11 +655,11 @@ static void launch_dkv(const Geometry &G, const void *q, const void *k, const vo
     f32x4 *slots = (f32x4 *)(ws + sp.slots_at);
     // floor(r * inv / 2^32) = r / group for r < kListed * group <= 2^20: inv is off by less than group / 2^32 of 1 / group
     const unsigned inv = G.group == 1 ? 0 : (unsigned)((0x100000000ULL + G.group - 1) / G.group);
-    hipLaunchKernelGGL((k_attend_dkv<T, DP, KW, KEYS, ROWS>), dim3((unsigned)(sp.max_items * sp.parts)), dim3(64 * KEYS * ROWS), 0, st, G,
+    hipLaunchKernelGGL((k_attend_dkv<T, DP, KW, KEYS, ROWS>), groups(sp.max_items * sp.parts), dim3(64 * KEYS * ROWS), 0, st, G,
                        (const T *)q, (const T *)k, (const T *)v, (const T *)dout, info, bits, items, n_items, slots, (T *)dk, (T *)dv, sp.words,
                        sp.parts, inv);
     if (sp.shared_out)
-        hipLaunchKernelGGL((k_join_dkv<T, DP, KW, KEYS, ROWS>), dim3((unsigned)(sp.max_items * sp.parts)), dim3(64 * KEYS), 0, st, G, items, n_items,
+        hipLaunchKernelGGL((k_join_dkv<T, DP, KW, KEYS, ROWS>), groups(sp.max_items * sp.parts), dim3(64 * KEYS), 0, st, G, items, n_items,
                            slots, (T *)dk, (T *)dv, sp.parts);
 }
 
@@ -673,16 +673,16 @@ static void launch_bwd(const Geometry &G, const void *q, const void *k, const vo
     if (G.q_rows > 0) {
         const int per_tile = G.group < 16 ? 16 / G.group : 1;
 #define NSP_GO(WIDE)                                                                                                                     \
-    hipLaunchKernelGGL((k_attend_dq<T, DP, WIDE>), dim3((unsigned)(ceil_div(G.q_rows, 4 * per_tile) * slices * G.kv_heads)), \
+    hipLaunchKernelGGL((k_attend_dq<T, DP, WIDE>), groups(ceil_div(G.q_rows, 4 * per_tile) * slices * G.kv_heads), \
                        dim3(256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx, (const T *)out, lse, (const T *)dout, (T *)dq,    \
                        info, slices, per_tile)
         if (G.block >= 32) NSP_GO(true); else NSP_GO(false);
 #undef NSP_GO
         if (sp.gms > 0) {
-            hipLaunchKernelGGL(k_pattern_bits, dim3((unsigned)((long long)sp.words * G.kv_heads)), dim3(256), 0, st, G, idx, bits, sp.words);
+            hipLaunchKernelGGL(k_pattern_bits, groups((long long)sp.words * G.kv_heads), dim3(256), 0, st, G, idx, bits, sp.words);
             if (sp.shared_out) {
                 int *counts = (int *)(ws + sp.counts_at);
-                hipLaunchKernelGGL(k_count_rows, dim3((unsigned)ceil_div(sp.gms, 4)), dim3(256), 0, st, G, bits, counts, sp.gms, sp.words);
+                hipLaunchKernelGGL(k_count_rows, groups(ceil_div(sp.gms, 4)), dim3(256), 0, st, G, bits, counts, sp.gms, sp.words);
                 hipLaunchKernelGGL(k_plan_items, dim3(1), dim3(1024), 0, st, counts, sp.gms, sp.per_item, (Item *)(ws + sp.items_at), counts + sp.gms);
             }
         }
@@ -726,7 +726,7 @@ int nsparse_lm_block_attention_bwd(const nsparse_lm_attn *a, const void *q, cons
     if (int rc = geometry(a, true, true, &G)) return rc;
     if (G.page_size > 0) return fail(NSPARSE_LM_EARG, "block_attention_bwd: not for paged caches");
     const BwdSpace sp = bwd_space(G);
-    if (sp.max_items * sp.parts > 0x7fffffffLL || (long long)sp.words * G.kv_heads > 0x7fffffffLL) return fail(NSPARSE_LM_EARG, "block_attention_bwd: blocks x heads out of range");
+    if (sp.max_items * sp.parts > kMostGroups) return fail(NSPARSE_LM_EARG, "block_attention_bwd: blocks x heads out of range");
     if ((G.q_rows > 0 && (!q || !idx || !out || !lse || !dout || !dq)) || (G.k_rows > 0 && (!k || !v || !dk || !dv)))
         return fail(NSPARSE_LM_EARG, "block_attention_bwd: a required pointer is NULL");
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv |

@@ -26,8 +26,8 @@ __global__ void __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256)
     const int lane = lane_id(), col = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     // consecutive workgroups go round the key heads: with 8 of them each XCD's cache serves one head's keys
-    const int g = (int)(blockIdx.x % G.kv_heads);
-    const int rest = (int)(blockIdx.x / G.kv_heads);
+    const int g = (int)(group_id() % G.kv_heads);
+    const int rest = (int)(group_id() / G.kv_heads);
     const int slice = rest % slices;
     const int t = WAVES > 1 ? rest / slices : (rest / slices) * 4 + wave;
     if (t >= G.q_rows) return;
@@ -202,8 +202,8 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
     __shared__ Union un;
     const int wave = uniform((int)(threadIdx.x >> 6));
     // consecutive workgroups go round the key heads: with 8 of them each XCD's cache serves one head's keys
-    const int g = (int)(blockIdx.x % G.kv_heads);
-    const int rest = (int)(blockIdx.x / G.kv_heads);
+    const int g = (int)(group_id() % G.kv_heads);
+    const int rest = (int)(group_id() / G.kv_heads);
     const int slice = rest % slices;
     const int per_wave = NT * per_tile;  // rows a wavefront
     const int t0 = (rest / slices) * 4 * per_wave;
@@ -390,7 +390,7 @@ static void launch_tiles(const Geometry &G, const void *q, const void *k, const 
 {
     const int slices = (int)ceil_div(G.group, 16);
     const int per_tile = G.group < 16 ? 16 / G.group : 1;
-    const dim3 grid((unsigned)(ceil_div(G.q_rows, 4 * NT * per_tile) * slices * G.kv_heads));
+    const dim3 grid = groups(ceil_div(G.q_rows, 4 * NT * per_tile) * slices * G.kv_heads);
     if (NG == 4 || G.block >= 16 * NG)
         hipLaunchKernelGGL((k_attend_tiles<T, DP, NT, NG, true>), grid, dim3(256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx,
                            (T *)out, lse, slices, per_tile);
@@ -424,7 +424,7 @@ static void launch_attend(const Geometry &G, const void *q, const void *k, const
         return;
     }
 #define NSP_GO(FULL, WAVES)                                                                                                          \
-    hipLaunchKernelGGL((k_attend<T, DP, NG, FULL, WAVES>), dim3((unsigned)((WAVES > 1 ? rows : ceil_div(G.q_rows, 4) * slices) * G.kv_heads)), \
+    hipLaunchKernelGGL((k_attend<T, DP, NG, FULL, WAVES>), groups((WAVES > 1 ? rows : ceil_div(G.q_rows, 4) * slices) * G.kv_heads), \
                        dim3(WAVES > 1 ? 64 * WAVES : 256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx, (T *)out, lse, slices)
     if (split) {
         constexpr int kSplit = DP * sizeof(T) > 512 ? 4 : 8;  // registers for a row's sums and a step's keys and values

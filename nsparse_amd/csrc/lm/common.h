@@ -15,6 +15,7 @@ void clear_error();
 int launched(const char *what);  // hipGetLastError as a return code
 
 inline int elem_size(int dtype) { return dtype == NSPARSE_LM_F32 ? 4 : 2; }
+constexpr long long kMostKeys = 0x7fffffffLL - 4096;  // of a sequence: a block's end is an int too
 inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // ---- types ---------------------------------------------------------------------------------------------------------
@@ -295,7 +296,7 @@ __device__ inline Seq seq_at(const Geometry &G, int s)
         q.k_base = 0;
         cap = G.k_rows > 0 ? G.table_stride * G.page_size : 0;
     } else if (G.cu_k) {
-        const int hi = (int)(G.k_rows < 0x7fffffffLL ? G.k_rows : 0x7fffffffLL);
+        const int hi = (int)G.k_rows;
         const int a = clampi(G.cu_k[s], 0, hi), b = clampi(G.cu_k[s + 1], a, hi);
         q.k_base = a;
         cap = b - a;
@@ -303,10 +304,16 @@ __device__ inline Seq seq_at(const Geometry &G, int s)
         q.k_base = (long long)s * G.k_each;
         cap = G.k_each;
     }
-    if (cap > 0x7fffffffLL) cap = 0x7fffffffLL;
+    if (cap > kMostKeys) cap = kMostKeys;
     q.k_len = G.k_len ? clampi(G.k_len[s], 0, (int)cap) : (int)cap;
     return q;
 }
+
+// Workgroups of a launch, counted through both dimensions of the grid: one dimension holds less than 2^32 threads.  There may be up
+// to kGridX - 1 more of them than asked for.
+constexpr long long kGridX = 1 << 21, kMostGroups = 0x7fffffffLL - kGridX;
+inline dim3 groups(long long n) { return n <= kGridX ? dim3((unsigned)n) : dim3((unsigned)kGridX, (unsigned)ceil_div(n, kGridX)); }
+__device__ inline unsigned group_id() { return blockIdx.y * gridDim.x + blockIdx.x; }
 
 // the sequence of query row t and the row's number inside it, or -1 where no sequence has it
 __device__ inline int seq_of_query(const Geometry &G, int t, Seq &q)

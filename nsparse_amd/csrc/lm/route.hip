@@ -180,8 +180,8 @@ template <class U>
 __global__ void __launch_bounds__(256)
     k_gather_tokens(const U *__restrict__ x, const int *__restrict__ place, int tokens, int top, int pieces, int per, U *__restrict__ xs)
 {
-    const int t = (int)blockIdx.x * (256 / per) + (int)threadIdx.x / per;
-    if (t >= tokens) return;
+    const unsigned t = group_id() * (256 / per) + threadIdx.x / per;
+    if (t >= (unsigned)tokens) return;
     const int *pl = place + (long long)t * top;
     for (int c = (int)threadIdx.x % per; c < pieces; c += per) {
         const U v = x[(long long)t * pieces + c];
@@ -197,8 +197,8 @@ __global__ void __launch_bounds__(256)
     k_combine_tokens(const T *__restrict__ y, const int *__restrict__ place, const float *__restrict__ w, int tokens, int top, int channels,
                      int per, T *__restrict__ out)
 {
-    const int t = (int)blockIdx.x * (256 / per) + (int)threadIdx.x / per;
-    if (t >= tokens) return;
+    const unsigned t = group_id() * (256 / per) + threadIdx.x / per;
+    if (t >= (unsigned)tokens) return;
     const long long e0 = (long long)t * top;
     for (int c = ((int)threadIdx.x % per) * V; c < channels; c += per * V) {
         float a[V] = {};
@@ -222,8 +222,8 @@ __global__ void __launch_bounds__(256)
                          int tokens, int top, int channels, int per, T *__restrict__ dy, float *__restrict__ dw)
 {
     __shared__ float sums[2][4];
-    const int t = (int)blockIdx.x * (256 / per) + (int)threadIdx.x / per;
-    if (t >= tokens) return;  // whole wavefronts; with per = 256 the whole workgroup
+    const unsigned t = group_id() * (256 / per) + threadIdx.x / per;
+    if (t >= (unsigned)tokens) return;  // whole wavefronts; with per = 256 the whole workgroup
     const long long e0 = (long long)t * top;
     const T *g = dout + (long long)t * channels;
     for (int j = 0; j < top; j++) {
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(256)
 static int check_products(int dtype, long long tokens, int top, int channels, const char *what)
 {
     if (dtype != NSPARSE_LM_F32 && dtype != NSPARSE_LM_F16 && dtype != NSPARSE_LM_BF16) return fail(NSPARSE_LM_ETYPE, "dtype is none of F32, F16, BF16");
-    if (tokens < 0 || top < 1 || channels < 1 || tokens > (0x7fffffffLL - 4096) / top) return fail(NSPARSE_LM_EARG, what);
+    if (tokens < 0 || top < 1 || channels < 1 || channels > 1 << 28 || tokens > (0x7fffffffLL - 4096) / top) return fail(NSPARSE_LM_EARG, what);
     return 0;
 }
 // threads a token: a wavefront for short rows, else a workgroup
@@ -317,9 +317,10 @@ int nsparse_lm_gather_tokens(int dtype, const void *x, const int *place, long lo
     if (!x || !place || !xs) return fail(NSPARSE_LM_EARG, "gather_tokens: a required pointer is NULL");
     const long long row = (long long)channels * elem_size(dtype);
     const int per = threads_per_token(channels, dtype);
-    const dim3 grid((unsigned)ceil_div(tokens, 256 / per));
+    const dim3 grid = groups(ceil_div(tokens, 256 / per));
     hipStream_t st = (hipStream_t)stream;
     const uintptr_t at = (uintptr_t)x | (uintptr_t)xs | (uintptr_t)row;
+    if (at % elem_size(dtype)) return fail(NSPARSE_LM_EALIGN, "gather_tokens: x and xs begin at elements of their type");
 #define NSP_GO(U)                                                                                                              \
     hipLaunchKernelGGL(k_gather_tokens<U>, grid, dim3(256), 0, st, (const U *)x, place, (int)tokens, top, (int)(row / sizeof(U)), per, (U *)xs)
     if (at % 16 == 0) NSP_GO(u32x4);
@@ -337,9 +338,10 @@ int nsparse_lm_combine_tokens(int dtype, const void *y, const int *place, const 
     if (int rc = check_products(dtype, tokens, top, channels, "combine_tokens: tokens, top or channels out of range")) return rc;
     if (tokens == 0) return 0;
     if (!y || !place || !out) return fail(NSPARSE_LM_EARG, "combine_tokens: a required pointer is NULL");
+    if (((uintptr_t)y | (uintptr_t)out) % elem_size(dtype)) return fail(NSPARSE_LM_EALIGN, "combine_tokens: y and out begin at elements of their type");
     const bool wide = (((uintptr_t)y | (uintptr_t)out | (uintptr_t)((long long)channels * elem_size(dtype))) & 15) == 0;
     const int per = threads_per_token(channels, dtype);
-    const dim3 grid((unsigned)ceil_div(tokens, 256 / per));
+    const dim3 grid = groups(ceil_div(tokens, 256 / per));
     hipStream_t st = (hipStream_t)stream;
 #define NSP_GO(T, V) \
     hipLaunchKernelGGL((k_combine_tokens<T, V>), grid, dim3(256), 0, st, (const T *)y, place, w, (int)tokens, top, channels, per, (T *)out)
@@ -358,9 +360,11 @@ int nsparse_lm_combine_tokens_bwd(int dtype, const void *dout, const void *y, co
     if (int rc = check_products(dtype, tokens, top, channels, "combine_tokens_bwd: tokens, top or channels out of range")) return rc;
     if (tokens == 0) return 0;
     if (!dout || !place || !dy || (dw && !y) || (w && !dw)) return fail(NSPARSE_LM_EARG, "combine_tokens_bwd: a required pointer is NULL");
+    if (((uintptr_t)dout | (uintptr_t)y | (uintptr_t)dy) % elem_size(dtype))
+        return fail(NSPARSE_LM_EALIGN, "combine_tokens_bwd: dout, y and dy begin at elements of their type");
     const bool wide = (((uintptr_t)dout | (uintptr_t)y | (uintptr_t)dy | (uintptr_t)((long long)channels * elem_size(dtype))) & 15) == 0;
     const int per = threads_per_token(channels, dtype);
-    const dim3 grid((unsigned)ceil_div(tokens, 256 / per));
+    const dim3 grid = groups(ceil_div(tokens, 256 / per));
     hipStream_t st = (hipStream_t)stream;
 #define NSP_GO(T, V)                                                                                                                 \
     hipLaunchKernelGGL((k_combine_tokens_bwd<T, V>), grid, dim3(256), 0, st, (const T *)dout, (const T *)y, place, w, (int)tokens, top, \

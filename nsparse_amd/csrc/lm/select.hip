@@ -16,11 +16,12 @@ template <class T>
 __global__ void __launch_bounds__(256) k_block_means(const Geometry G, const T *__restrict__ k, T *__restrict__ means, int last, int per_seq)
 {
     __shared__ double part[256 * 8];
-    const int g = (int)(blockIdx.x % G.kv_heads);
-    const long long rest = blockIdx.x / G.kv_heads;
+    const int g = (int)(group_id() % G.kv_heads);
+    const long long rest = group_id() / G.kv_heads;
     Seq sq;
     int b;
     if (per_seq > 0) {
+        if (rest / per_seq >= G.n_seq) return;
         sq = seq_at(G, (int)(rest / per_seq));
         b = (int)(rest % per_seq);
         if (last > 0) b += (sq.k_len > last ? sq.k_len - last : 0) / G.block;
@@ -353,9 +354,11 @@ __global__ void __launch_bounds__(256)
     __shared__ Plain pl;
     const int lane = lane_id(), col = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int g = (int)((gridDim.x - 1 - blockIdx.x) % G.kv_heads);
+    const int all = (G.q_rows + 15) / 16 * G.kv_heads, mine = all - 1 - (int)group_id();
+    if (mine < 0) return;
+    const int g = mine % G.kv_heads;
     // the last rows, which see most, begin first
-    const int t0 = (int)((gridDim.x - 1 - blockIdx.x) / G.kv_heads) * 16;
+    const int t0 = mine / G.kv_heads * 16;
     const int t1 = t0 + 16 < G.q_rows ? t0 + 16 : G.q_rows;
     if (threadIdx.x < 16) plain_row[threadIdx.x] = 0;
     // the group's summed queries, and the norm of the sum of their absolute values
@@ -464,7 +467,8 @@ __global__ void __launch_bounds__(1024)
     __shared__ Plain pl;
     const int lane = lane_id(), l16 = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int g = (int)(blockIdx.x % G.kv_heads), t = (int)(blockIdx.x / G.kv_heads);
+    const int g = (int)(group_id() % G.kv_heads), t = (int)(group_id() / G.kv_heads);
+    if (t >= G.q_rows) return;
     Seq sq;
     const int i = seq_of_query(G, t, sq);
     if (i < 0) return;
@@ -554,7 +558,8 @@ __global__ void __launch_bounds__(256)
 {
     __shared__ __align__(16) char space[12 * 4096];
     __shared__ Plain pl;
-    const int g = (int)(blockIdx.x % G.kv_heads), t = (int)(blockIdx.x / G.kv_heads);
+    const int g = (int)(group_id() % G.kv_heads), t = (int)(group_id() / G.kv_heads);
+    if (t >= G.q_rows) return;
     Seq sq;
     const int i = seq_of_query(G, t, sq);
     if (i < 0) return;
@@ -566,7 +571,7 @@ __global__ void __launch_bounds__(256)
 template <class T, int KS>
 static void launch_rows(const Geometry &G, long long blocks, int first, int local, const void *q, const void *means, int *idx, hipStream_t st)
 {
-    const dim3 grid((unsigned)(ceil_div(G.q_rows, 16) * G.kv_heads));
+    const dim3 grid = groups(ceil_div(G.q_rows, 16) * G.kv_heads);
     if (blocks <= 256)
         hipLaunchKernelGGL((k_select_rows<T, KS, 256>), grid, dim3(256), 0, st, G, first, local, (const T *)q, (const T *)means, idx);
     else if (blocks <= 768)
@@ -586,7 +591,7 @@ static void launch_select(const Geometry &G, int first, int local, const void *q
         else launch_rows<T, 8>(G, blocks, first, local, q, means, idx, st);
         return;
     }
-    const dim3 grid((unsigned)((long long)G.q_rows * G.kv_heads));
+    const dim3 grid = groups((long long)G.q_rows * G.kv_heads);
     if (blocks <= kOneCap) {
         // the plain way wants 32 KB
         const size_t lds = blocks <= 8192 ? 8192 * 4 : (size_t)blocks * 4;
@@ -619,9 +624,9 @@ int nsparse_lm_block_means(const nsparse_lm_attn *a, const void *k, void *means,
     if (last > 0) per_seq = (last - 1) / G.block + 2;
     if (G.page_size > 0 && (per_seq == 0 || per_seq > G.table_stride * G.per_page)) per_seq = G.table_stride * G.per_page;
     rows = per_seq > 0 ? per_seq * G.n_seq : nsparse_lm_mean_rows(a);
-    if (rows * G.kv_heads > 0x7fffffffLL) return fail(NSPARSE_LM_EARG, "block_means: blocks x heads out of range");
+    if (rows * G.kv_heads > kMostGroups) return fail(NSPARSE_LM_EARG, "block_means: blocks x heads out of range");
     if (rows == 0) return 0;
-    const dim3 grid((unsigned)(rows * G.kv_heads));
+    const dim3 grid = groups(rows * G.kv_heads);
     hipStream_t st = (hipStream_t)stream;
     if (a->dtype == NSPARSE_LM_BF16)
         hipLaunchKernelGGL(k_block_means<__bf16>, grid, dim3(256), 0, st, G, (const __bf16 *)k, (__bf16 *)means, last, (int)per_seq);

@@ -38,6 +38,11 @@ class Seqs:
         if page_table is not None and (page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != self.n
                                        or page_table.stride(1) != 1 and page_table.shape[1] > 1):
             raise ValueError("Seqs: page_table must be an int32 tensor [n, pages] with contiguous rows")
+        # a table cut out of a wider one: its rows count as long as they are apart, so the last one has to be there in full
+        if page_table is not None and self.n > 1 and (
+                page_table.stride(0) < page_table.shape[1] or
+                page_table.storage_offset() + self.n * page_table.stride(0) > page_table.untyped_storage().nbytes() // 4):
+            raise ValueError("Seqs: page_table's rows must not overlap, and a cut of a wider table must keep the last row's end")
         self.cu_q, self.cu_k, self.q_len, self.k_len, self.page_table = cu_q, cu_k, q_len, k_len, page_table
 
     # addresses, read at every call (0: none)
@@ -127,11 +132,14 @@ def _attn(seqs, block, *, q=None, k=None, v=None, kv_heads=None, k_rows=None, pa
             raise ValueError("q, k and v must have one head_dim and type")
         if table is not None:
             page_size = shape[1]
-    a = LmAttn.from_buffer_copy(_ATTN.pack(
-        dtype, heads, kv_heads, dim, int(block), int(width), 1 if causal else 0, seqs.n, page_size, int(first), int(local), scale, q_rows,
-        int(k_rows), 0 if table is None else (table.stride(0) if seqs.n > 1 else table.shape[1]), 0 if q is None else seqs.ptr_cu_q,
-        seqs.ptr_cu_k, 0 if q is None else seqs.ptr_q_len, seqs.ptr_k_len, seqs.ptr_table, q0, q1, *ks, *vs))
-    return a, kv_heads
+    try:
+        packed = _ATTN.pack(
+            dtype, heads, kv_heads, dim, int(block), int(width), 1 if causal else 0, seqs.n, page_size, int(first), int(local), scale, q_rows,
+            int(k_rows), 0 if table is None else (table.stride(0) if seqs.n > 1 else table.shape[1]), 0 if q is None else seqs.ptr_cu_q,
+            seqs.ptr_cu_k, 0 if q is None else seqs.ptr_q_len, seqs.ptr_k_len, seqs.ptr_table, q0, q1, *ks, *vs)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"an argument is out of range: {e}") from None
+    return LmAttn.from_buffer_copy(packed), kv_heads
 
 
 def _key_strides(t, what, paged):
