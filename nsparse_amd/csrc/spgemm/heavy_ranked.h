@@ -91,7 +91,7 @@ __global__ __launch_bounds__(BS) void k_num_ranked(const int *__restrict__ arpt,
             s_nlong = 0;
         }
         __syncthreads();
-        const int q = s_row;
+        const int q = __builtin_amdgcn_readfirstlane(s_row);  // uniform: what hangs on the row needs no vector registers
         if (q >= count) break;
         const int rid = row_perm[bin_off + q];
         const int lo = row_lo[rid], span = row_span[rid];
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(BS) void k_num_ranked(const int *__restrict__ arpt,
             st_av[e] = av;
         }
         __syncthreads();
-        const int nlong = s_nlong < LCAP ? s_nlong : LCAP;
+        const int nlong = __builtin_amdgcn_readfirstlane(s_nlong < LCAP ? s_nlong : LCAP);
         const int row_end = lo + span;
         int t_lo = lo;
         int sym_cnt = 0;
@@ -448,7 +448,7 @@ __global__ __launch_bounds__(BS) void k_num_ranked(const int *__restrict__ arpt,
             }
             lds_barrier();
             }  // pass 1 + scan (rows without a list)
-            const int t_hi = rlist ? t_hi_l : s_cut, ntile = rlist ? ntile_l : s_ntile;
+            const int t_hi = __builtin_amdgcn_readfirstlane(rlist ? t_hi_l : s_cut), ntile = __builtin_amdgcn_readfirstlane(rlist ? ntile_l : s_ntile);
             tick(2);
             if (kExperiments && prof && t_hi != t_max) t_acc[9]++;
             walk(std::true_type{}, t_hi);
