@@ -5,11 +5,14 @@
   * tokens sorted by expert and back: route, gather_tokens, combine_tokens (both differentiable) and their *_backward.
 
 Tensors live on one GPU; work is queued on that device's current stream and nothing synchronises, so every call may be captured
-into a graph.  Refused arguments raise ValueError with the reason.  There is no fallback: a missing library raises.
+into a graph.  A backward pass is captured by calling the *_backward functions, or through autograd while no graph made outside of the
+capture over the same leaves is alive (refused with RuntimeError where such a graph came from these functions).  Refused
+arguments raise ValueError with the reason.  There is no fallback: a missing library raises.
 """
 import ctypes as C
 import math
 import struct
+import weakref
 
 import torch
 
@@ -230,9 +233,26 @@ def _attention(dev, q, k, v, idx, block, scale, causal, seqs, out, lse):
     return out, lse
 
 
+# Autograd nodes that were made outside of a capture and are alive.  A leaf's gradient is accumulated on the stream on which the first
+# of its living nodes was made: a backward pass captured while one of these lives would leave the capture, which ends the process.
+_eager = weakref.WeakSet()
+
+
+def _may_capture(ctx, *inputs):
+    ctx.leaves = [id(t) for t in inputs if t.requires_grad and t.is_leaf]
+    if not ctx.leaves:
+        return
+    if torch.cuda.is_current_stream_capturing():
+        if any(x in node.leaves for node in list(_eager) for x in ctx.leaves):
+            raise RuntimeError("a graph made outside of this capture over the same leaves is alive: delete its outputs before capturing")
+    else:
+        _eager.add(ctx)
+
+
 class _BlockAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, idx, block, scale, causal, seqs):
+        _may_capture(ctx, q, k, v)
         out, lse = _attention(q.get_device(), q, k, v, idx, block, scale, causal, seqs, None, None)
         ctx.save_for_backward(q, k, v, idx, out, lse, *seqs._tensors())
         ctx.rest = (block, scale, causal, seqs)
@@ -358,6 +378,7 @@ def _combine(y, plan, weights):
 class _Gather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, plan):
+        _may_capture(ctx, x)
         ctx.plan = plan
         return _gather(x, plan)
 
@@ -370,6 +391,7 @@ class _Gather(torch.autograd.Function):
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, plan, weights):
+        _may_capture(ctx, y, weights)
         ctx.plan = plan
         ctx.save_for_backward(y, weights)
         return _combine(y, plan, weights)
@@ -396,6 +418,8 @@ def gather_tokens_backward(dxs, plan):
 
 def combine_tokens(y, plan, weights):
     """out [tokens, channels] = sum over a token's entries of weights [tokens, top] (float32) times their rows of y.  Differentiable."""
+    if weights is None:
+        raise ValueError("weights must be given; a plain sum of a token's rows is gather_tokens_backward")
     if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad):
         return _Combine.apply(y, plan, weights)
     return _combine(y, plan, weights)
