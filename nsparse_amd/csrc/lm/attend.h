@@ -293,8 +293,15 @@ template <class T, int DP> __device__ inline void store_row(T *p, const f32x4 (&
         }
     }
 }
-// A step's keys (or values) to LDS, by 256 threads.  Whole tiles go there straight from memory (the wait is the barrier's); tiles with
-// keys that nobody sees, or rows shorter than DP, through registers, with zeros for what is not there.
+// 16 bytes a lane from memory to LDS without registers: lane i's land at the wavefront's `to` + 16 i, the wait is the next barrier's.
+// What is not there (behind head_dim, rows that nobody sees) comes from 16 bytes of zeros.
+static __device__ const u32x4 kNothing[1] = {};
+__device__ inline void fetch(u32x4 *to, const void *from, bool there)
+{
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(there ? from : kNothing),
+                                     (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+// A step's keys (or values) to LDS, by 256 threads.
 template <class T, int DP, int NG, bool WIDE>
 __device__ inline void tile_load(u32x4 *t, const T *p, const long long (&off)[WIDE ? 1 : NG], const Step<NG, WIDE> &s, long long stride, int head_dim)
 {
@@ -304,9 +311,6 @@ __device__ inline void tile_load(u32x4 *t, const T *p, const long long (&off)[WI
     static_assert(kRows <= 16 || kRows % 16 == 0, "a pass covers whole groups or a part of one");
     const int tid = opaque((int)threadIdx.x);
     const int at = tid % kPieces, r0 = tid / kPieces;
-    bool whole = head_dim == DP;
-#pragma unroll
-    for (int y = 0; y < NG; y++) whole = whole && s.rows(y) >= 16;
 #pragma unroll
     for (int i = 0; i < kPasses; i++) {
         const int r = r0 + i * kRows, y0 = i * kRows / 16;
@@ -327,15 +331,7 @@ __device__ inline void tile_load(u32x4 *t, const T *p, const long long (&off)[WI
                 }
             o += (long long)(r & 15) * stride + c;
         }
-        if (whole) {
-            // lane i's 16 bytes land at the wavefront's base + 16 i
-            u32x4 *base = t + i * 256 + uniform(tid & ~63);
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(p + o), (__attribute__((address_space(3))) void *)base, 16, 0, 0);
-        } else {
-            u32x4 x = u32x4{0, 0, 0, 0};
-            if ((r & 15) < n && c < head_dim) x = *(const u32x4 *)(p + o);
-            t[i * 256 + tid] = x;
-        }
+        fetch(t + i * 256 + uniform(tid & ~63), p + o, (r & 15) < n && c < head_dim);
     }
 }
 

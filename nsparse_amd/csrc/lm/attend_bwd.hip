@@ -437,7 +437,6 @@ __global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>:
         auto prepare = [&](int step, int buf) {
             const int o = opaque(tid);
             const int r0 = step * kStep;
-            const bool whole = D == DP && r0 + kStep <= rows;
 #pragma unroll
             for (int i = 0; i < C::kTile / kThreads; i++) {
                 const int x = i * kThreads + o, r = x / kPieces, rr = r0 + r;
@@ -446,21 +445,9 @@ __global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>:
                 const int ti = token_of(in ? rr : 0), hh = g * G.group + ((in ? rr : 0) - ti * G.group);
                 const long long t = list[ti];
                 const T *pq = q + t * G.q_row + (long long)hh * G.q_head + c, *pg = dout + (t * G.heads + hh) * D + c;
-                if (whole) {
-                    const int base = i * kThreads + uniform(o & ~63);
-                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)pq,
-                                                     (__attribute__((address_space(3))) void *)(qt(buf) + base), 16, 0, 0);
-                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)pg,
-                                                     (__attribute__((address_space(3))) void *)(gt(buf) + base), 16, 0, 0);
-                } else {
-                    u32x4 y = u32x4{0, 0, 0, 0}, z = y;
-                    if (in && c < D) {
-                        y = *(const u32x4 *)pq;
-                        z = *(const u32x4 *)pg;
-                    }
-                    qt(buf)[x] = y;
-                    gt(buf)[x] = z;
-                }
+                const int to = i * kThreads + uniform(o & ~63);
+                fetch(qt(buf) + to, pq, in && c < D);
+                fetch(gt(buf) + to, pg, in && c < D);
             }
         };
         if (steps > 0) {
@@ -605,12 +592,21 @@ __global__ void __launch_bounds__(64 * KEYS)
     const int kw = uniform((int)(threadIdx.x >> 6)), lane = lane_id();
     typename C::Sums a;
     const f32x4 *p = slots + (((long long)it.slot * parts + part) * KEYS + kw) * C::kDump * 64 + lane;
+    const long long apart = (long long)parts * KEYS * C::kDump * 64;
 #pragma unroll
     for (int x = 0; x < C::kDump; x++) a.at(x) = p[x * 64];
-    for (int c = 1; c < it.chunks; c++) {
-        p += (long long)parts * KEYS * C::kDump * 64;
+    // a few items' sums are on their way at a time
+    constexpr int kAhead = C::kDump <= 16 ? 4 : 2;
+    for (int c = 1; c < it.chunks; c += kAhead) {
+        f32x4 w[kAhead][C::kDump];
 #pragma unroll
-        for (int x = 0; x < C::kDump; x++) a.at(x) += p[x * 64];
+        for (int u = 0; u < kAhead; u++)
+#pragma unroll
+            for (int x = 0; x < C::kDump; x++) w[u][x] = c + u < it.chunks ? p[(c + u) * apart + x * 64] : f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int u = 0; u < kAhead; u++)
+#pragma unroll
+            for (int x = 0; x < C::kDump; x++) a.at(x) += w[u][x];
     }
     C::store(G, a, sq, b, it.gm % G.kv_heads, part, kw, dk, dv);
 }

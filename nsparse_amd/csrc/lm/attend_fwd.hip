@@ -289,6 +289,11 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
                             });
 #pragma unroll
                         for (int x = 0; x < NT; x++) {
+                            if (NT > 1 && !((st.any >> ((wave * NT + x) * per_tile)) & ((1ULL << per_tile) - 1))) {
+#pragma unroll
+                                for (int y = 0; y < NG; y += 2) pf[x][y / 2] = frag_zero<T>();
+                                continue;
+                            }
                             bool on[NG];
                             bool all = WIDE;
 #pragma unroll
