@@ -437,6 +437,7 @@ __global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>:
         auto prepare = [&](int step, int buf) {
             const int o = opaque(tid);
             const int r0 = step * kStep;
+            const bool whole = D == DP && r0 + kStep <= rows;
 #pragma unroll
             for (int i = 0; i < C::kTile / kThreads; i++) {
                 const int x = i * kThreads + o, r = x / kPieces, rr = r0 + r;
@@ -446,8 +447,13 @@ __global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>:
                 const long long t = list[ti];
                 const T *pq = q + t * G.q_row + (long long)hh * G.q_head + c, *pg = dout + (t * G.heads + hh) * D + c;
                 const int to = i * kThreads + uniform(o & ~63);
-                fetch(qt(buf) + to, pq, in && c < D);
-                fetch(gt(buf) + to, pg, in && c < D);
+                if (whole) {
+                    fetch(qt(buf) + to, pq, true);
+                    fetch(gt(buf) + to, pg, true);
+                } else {
+                    fetch(qt(buf) + to, pq, in && c < D);
+                    fetch(gt(buf) + to, pg, in && c < D);
+                }
             }
         };
         if (steps > 0) {
