@@ -284,8 +284,8 @@ __global__ void __launch_bounds__(1024)
 // products, and ROWS of them one behind the other, each with its own 32 of the (query, head) pairs that list the block.
 // The pairs' rows of q and dout go through LDS (by rows for S = Q K^T and dP = dO V^T, transposed for dK^T = Q^T dS and
 // dV^T = dO^T P), fetched while the 32 before are computed.  Bound by what LDS delivers: the more keys a wavefront, the fewer reads a product.
-// 4096 rows of 32 query and 8 key heads of 128, 16 blocks of 64 each, bf16: 225 us, and 27 for the join of the shared-out blocks' sums; the
-// transposed pattern takes 5 us, counting and planning 5 each.
+// 4096 rows of 32 query and 8 key heads of 128, 16 blocks of 64 each, bf16: 228 us, and 22 for the join of the shared-out blocks' sums; the
+// transposed pattern takes 5 us, counting and planning 5 each.  1501 fp32 rows of 6 and 2 heads of 96, 12 blocks of 16 each: 95 and 10 us.
 constexpr int kItems = 1024;
 constexpr int kListed = 1024;
 template <class T, int DP, int KW, int KEYS, int ROWS> struct Dkv {
@@ -437,6 +437,7 @@ __global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>:
         auto prepare = [&](int step, int buf) {
             const int o = opaque(tid);
             const int r0 = step * kStep;
+            // (asking for whole tiles without the choice: 228 against 240 us)
             const bool whole = D == DP && r0 + kStep <= rows;
 #pragma unroll
             for (int i = 0; i < C::kTile / kThreads; i++) {

@@ -12,7 +12,7 @@
 // once, into LDS, while the block before is computed.
 // With few rows (a serving step) eight wavefronts share a row: wavefront w takes every eighth tile of keys and the partial
 // results meet in LDS.
-// Measured, 32 query and 8 key heads of 128, 16 blocks of 64, bf16.  8192 rows of a prompt whose neighbours agree on part of their blocks: 435 us, 283 TFLOP/s
+// Measured, 32 query and 8 key heads of 128, 16 blocks of 64, bf16.  8192 rows of a prompt whose neighbours agree on part of their blocks: 402 us, 311 TFLOP/s
 // over the listed keys; bound by LDS (a wavefront reads as many cycles of operands as its products take) and by blocks that only
 // some of the workgroup's rows list.  64 conversations, one row each, 32 blocks: 46 us, 4.2 TB/s, bound by memory.  One row: 15 us, bound by latency.
 #include "attend.h"
@@ -419,12 +419,12 @@ static void launch_attend(const Geometry &G, const void *q, const void *k, const
     // neighbouring rows together where there are some (256 sequences of 3 new tokens: 357 against 297 us row by row, of 4: 224;
     // but 512 of 2, 2 heads each and blocks of 16: 57 against 200)
     if (!split && G.q_rows / G.n_seq >= 4) {
-        // 64 keys a step where a block has them, else 32 (blocks of 32 in steps of 64: 58 against 39 us for 3945 rows of 16 heads)
+        // 64 keys a step where a block has them, else 32 (blocks of 32 in steps of 64: 55 against 39 us for 3945 rows of 16 heads)
         const int per_tile = G.group < 16 ? 16 / G.group : 1;
         if constexpr (sizeof(T) == 2 && DP <= 128) {
             if (G.block >= 64) {
-                // two sets of columns read half as much of LDS a product, but neighbours have to agree on more blocks (8192 rows, 32/8 heads: 487 against
-                // 603 us with one set where few agree, 336 against 291 where sixteen rows agree on all but one; 2048 rows, 64/4 heads: 99 against 117)
+                // two sets of columns read half as much of LDS a product, but neighbours have to agree on more blocks (8192 rows, 32/8 heads: 442 against
+                // 549 us with one set where few agree, 305 against 274 where sixteen rows agree on all but one; 2048 rows, 64/4 heads: 92 against 111)
                 if (per_tile <= 8 && rows * G.kv_heads >= 2 * per_tile * 2048LL) launch_tiles<T, DP, 2, 4>(G, q, k, v, idx, out, lse, st);
                 else launch_tiles<T, DP, 1, 4>(G, q, k, v, idx, out, lse, st);
                 return;
