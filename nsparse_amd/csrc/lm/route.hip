@@ -5,7 +5,7 @@
 //   rows of smaller experts + the expert's rows of earlier chunks + of earlier wavefronts + of earlier lanes,
 // each a count of what stands before it, so no atomic decides an order.  The products with the matrix are one pass over the token
 // rows; every kernel works token by token: the token's row stays in registers or cache while its `top` rows are read or written.
-// All of it is bound by memory: gather and combine of 16384 x 4096 bf16 rows, 8 entries each, 251 and 275 us, the gradient of combine 479 (1.2, 1.2
+// All of it is bound by memory: gather and combine of 16384 x 4096 bf16 rows, 8 entries each, 250 and 272 us, the gradient of combine 462 (1.2, 1.2
 // and 2.3 GB; a large copy reaches 4.8 TB/s); sorting 131072 entries 13 us in three launches, up to 4096 entries 6 us in one.
 #include "common.h"
 
@@ -147,57 +147,63 @@ __global__ void __launch_bounds__(1024)
 }
 
 // ---- products with the routing matrix -----------------------------------------------------------------------------------
-// A row is read in pieces of V elements (16 bytes where sizes and addresses allow, else one element).
-template <class T, int V> struct Piece;
-template <class T> struct Piece<T, 1> {
-    static __device__ inline void load(const T *p, float *x) { x[0] = to_f32(*p); }
-    static __device__ inline void store(T *p, const float *x) { *p = from_f32<T>(x[0]); }
-};
-template <class T> struct Piece<T, 8> {
-    static __device__ inline void load(const T *p, float *x)
+// A row is read in pieces of 16 bytes, V elements, the last one element by element where it is shorter.  Rows of odd sizes begin at any element:
+// memory takes pieces from there too (1003 fp32 rows of 1023, 3 entries each, against element by element: combine 6 and 10 us, gather 5 and 7).
+template <class T> struct Piece {
+    static constexpr int V = 16 / (int)sizeof(T);
+    typedef __attribute__((ext_vector_type(V))) T Vec;
+    struct __attribute__((packed, aligned(sizeof(T)))) Loose { Vec v; };
+    static __device__ inline Vec load(const T *p, int n)
     {
-        typedef __attribute__((ext_vector_type(8))) T T8;
-        const T8 v = *(const T8 *)p;
+        if (n >= V) return ((const Loose *)p)->v;
+        Vec v{};
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = (float)v[i];
+        for (int i = 0; i < V; i++)
+            if (i < n) v[i] = p[i];
+        return v;
     }
-    static __device__ inline void store(T *p, const float *x)
+    static __device__ inline void store(T *p, const Vec &v, int n)
     {
-        *(u32x4 *)p = u32x4{pack2(x[0], x[1], T{}), pack2(x[2], x[3], T{}), pack2(x[4], x[5], T{}), pack2(x[6], x[7], T{})};
-    }
-};
-template <> struct Piece<float, 4> {
-    static __device__ inline void load(const float *p, float *x)
-    {
-        const f32x4 v = *(const f32x4 *)p;
+        if (n >= V) {
+            ((Loose *)p)->v = v;
+            return;
+        }
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = v[i];
+        for (int i = 0; i < V; i++)
+            if (i < n) p[i] = v[i];
     }
-    static __device__ inline void store(float *p, const float *x) { *(f32x4 *)p = f32x4{x[0], x[1], x[2], x[3]}; }
+    static __device__ inline Vec round(const float (&x)[V])
+    {
+        Vec v;
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = from_f32<T>(x[i]);
+        return v;
+    }
 };
 
-// U: the unsigned type of V elements, moved as bits
+// U: an unsigned type of the elements' size, moved as bits
 template <class U>
 __global__ void __launch_bounds__(256)
-    k_gather_tokens(const U *__restrict__ x, const int *__restrict__ place, int tokens, int top, int pieces, int per, U *__restrict__ xs)
+    k_gather_tokens(const U *__restrict__ x, const int *__restrict__ place, int tokens, int top, int channels, int per, U *__restrict__ xs)
 {
     const unsigned t = group_id() * (256 / per) + threadIdx.x / per;
     if (t >= (unsigned)tokens) return;
     const int *pl = place + (long long)t * top;
-    for (int c = (int)threadIdx.x % per; c < pieces; c += per) {
-        const U v = x[(long long)t * pieces + c];
+    for (int c = ((int)threadIdx.x % per) * Piece<U>::V; c < channels; c += per * Piece<U>::V) {
+        const auto v = Piece<U>::load(x + (long long)t * channels + c, channels - c);
         for (int j = 0; j < top; j++) {
             const int p = pl[j];
-            if (p >= 0) xs[(long long)p * pieces + c] = v;
+            if (p >= 0) Piece<U>::store(xs + (long long)p * channels + c, v, channels - c);
         }
     }
 }
 
-template <class T, int V>
+template <class T>
 __global__ void __launch_bounds__(256)
     k_combine_tokens(const T *__restrict__ y, const int *__restrict__ place, const float *__restrict__ w, int tokens, int top, int channels,
                      int per, T *__restrict__ out)
 {
+    constexpr int V = Piece<T>::V;
     const unsigned t = group_id() * (256 / per) + threadIdx.x / per;
     if (t >= (unsigned)tokens) return;
     const long long e0 = (long long)t * top;
@@ -207,53 +213,75 @@ __global__ void __launch_bounds__(256)
         for (int j = 0; j < top; j++) {
             const int p = place[e0 + j];
             if (p < 0) continue;
-            float x[V];
-            Piece<T, V>::load(y + (long long)p * channels + c, x);
+            const auto x = Piece<T>::load(y + (long long)p * channels + c, channels - c);
             const float f = w ? w[e0 + j] : 1.f;
 #pragma unroll
-            for (int i = 0; i < V; i++) a[i] += f * x[i];
+            for (int i = 0; i < V; i++) a[i] += f * (float)x[i];
         }
-        Piece<T, V>::store(out + (long long)t * channels + c, a);
+        Piece<T>::store(out + (long long)t * channels + c, Piece<T>::round(a), channels - c);
     }
 }
 
-template <class T, int V>
+template <class T>
 __global__ void __launch_bounds__(256)
     k_combine_tokens_bwd(const T *__restrict__ dout, const T *__restrict__ y, const int *__restrict__ place, const float *__restrict__ w,
                          int tokens, int top, int channels, int per, T *__restrict__ dy, float *__restrict__ dw)
 {
-    __shared__ float sums[2][4];
+    constexpr int V = Piece<T>::V;
+    constexpr int J = 4;  // entries at a time: their rows are on their way together, dout is read once for them
+    __shared__ float sums[2][4][J];
     const unsigned t = group_id() * (256 / per) + threadIdx.x / per;
     if (t >= (unsigned)tokens) return;  // whole wavefronts; with per = 256 the whole workgroup
     const long long e0 = (long long)t * top;
     const T *g = dout + (long long)t * channels;
-    for (int j = 0; j < top; j++) {
-        const int p = place[e0 + j];
-        float dot = 0.f;
-        if (p >= 0) {
-            const float f = w ? w[e0 + j] : 1.f;
-            for (int c = ((int)threadIdx.x % per) * V; c < channels; c += per * V) {
-                float a[V], x[V];
-                Piece<T, V>::load(g + c, a);
-                if (dw) {
-                    Piece<T, V>::load(y + (long long)p * channels + c, x);
+    for (int j0 = 0; j0 < top; j0 += J) {
+        int p[J];
+        float f[J], dot[J];
 #pragma unroll
-                    for (int i = 0; i < V; i++) dot += a[i] * x[i];
+        for (int j = 0; j < J; j++) {
+            const bool in = j0 + j < top;
+            p[j] = in ? place[e0 + j0 + j] : -1;
+            f[j] = in && w ? w[e0 + j0 + j] : 1.f;
+            dot[j] = 0.f;
+        }
+        for (int c = ((int)threadIdx.x % per) * V; c < channels; c += per * V) {
+            const auto a = Piece<T>::load(g + c, channels - c);
+            typename Piece<T>::Vec x[J];
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                x[j] = typename Piece<T>::Vec{};
+                if (dw && p[j] >= 0) x[j] = Piece<T>::load(y + (long long)p[j] * channels + c, channels - c);
+            }
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                if (p[j] < 0) continue;
+                float b[V];
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    dot[j] += (float)a[i] * (float)x[j][i];
+                    b[i] = (float)a[i] * f[j];
                 }
-#pragma unroll
-                for (int i = 0; i < V; i++) a[i] *= f;
-                Piece<T, V>::store(dy + (long long)p * channels + c, a);
+                Piece<T>::store(dy + (long long)p[j] * channels + c, Piece<T>::round(b), channels - c);
             }
         }
         if (!dw) continue;
 #pragma unroll
-        for (int d = 32; d > 0; d >>= 1) dot += __shfl_xor(dot, d);
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) dot[j] += __shfl_xor(dot[j], d);
+        const int left = top - j0 < J ? top - j0 : J;
+        float(*part)[J] = sums[(j0 / J) & 1];  // the other half is free until the next entries
         if (per == 64) {
-            if (lane_id() == 0) dw[e0 + j] = dot;
+#pragma unroll
+            for (int j = 0; j < J; j++)
+                if (lane_id() == j && j < left) dw[e0 + j0 + j] = dot[j];
         } else {
-            if (lane_id() == 0) sums[j & 1][threadIdx.x >> 6] = dot;
-            __syncthreads();  // the other half of `sums` is free until the next one
-            if (threadIdx.x == 0) dw[e0 + j] = sums[j & 1][0] + sums[j & 1][1] + sums[j & 1][2] + sums[j & 1][3];
+#pragma unroll
+            for (int j = 0; j < J; j++)
+                if (lane_id() == j) part[threadIdx.x >> 6][j] = dot[j];
+            __syncthreads();
+            const int j = (int)threadIdx.x;
+            if (j < left) dw[e0 + j0 + j] = part[0][j] + part[1][j] + part[2][j] + part[3][j];
         }
     }
 }
@@ -265,8 +293,8 @@ static int check_products(int dtype, long long tokens, int top, int channels, co
     return 0;
 }
 // threads a token: a wavefront for rows of at most 2 KB, whose pieces leave half a workgroup without work, else a workgroup.  Gradient of
-// combine, bf16, by wavefront against by workgroup: 16384 tokens of 1024 channels, 4 entries each: 62 and 92 us, of 512: 26 and 52; 8192 of
-// 4096: 122 and 129; 2048 of 2048: 18 and 14; 256 of 4096, 8 entries each: 39 and 17.
+// combine, bf16, by wavefront against by workgroup: 16384 tokens of 1024 channels, 4 entries each: 52 and 69 us, of 512: 27 and 44; 8192 of
+// 2048: 59 and 53, of 4096: 141 and 129; 256 of 4096, 8 entries each: 25 and 10.
 static int threads_per_token(int channels, int dtype) { return (long long)channels * elem_size(dtype) <= 2048 ? 64 : 256; }
 
 }  // namespace lm
@@ -318,16 +346,13 @@ int nsparse_lm_gather_tokens(int dtype, const void *x, const int *place, long lo
     if (int rc = check_products(dtype, tokens, top, channels, "gather_tokens: tokens, top or channels out of range")) return rc;
     if (tokens == 0) return 0;
     if (!x || !place || !xs) return fail(NSPARSE_LM_EARG, "gather_tokens: a required pointer is NULL");
-    const long long row = (long long)channels * elem_size(dtype);
+    if (((uintptr_t)x | (uintptr_t)xs) % elem_size(dtype)) return fail(NSPARSE_LM_EALIGN, "gather_tokens: x and xs begin at elements of their type");
     const int per = threads_per_token(channels, dtype);
     const dim3 grid = groups(ceil_div(tokens, 256 / per));
     hipStream_t st = (hipStream_t)stream;
-    const uintptr_t at = (uintptr_t)x | (uintptr_t)xs | (uintptr_t)row;
-    if (at % elem_size(dtype)) return fail(NSPARSE_LM_EALIGN, "gather_tokens: x and xs begin at elements of their type");
-#define NSP_GO(U)                                                                                                              \
-    hipLaunchKernelGGL(k_gather_tokens<U>, grid, dim3(256), 0, st, (const U *)x, place, (int)tokens, top, (int)(row / sizeof(U)), per, (U *)xs)
-    if (at % 16 == 0) NSP_GO(u32x4);
-    else if (at % 4 == 0) NSP_GO(unsigned);
+#define NSP_GO(U) \
+    hipLaunchKernelGGL(k_gather_tokens<U>, grid, dim3(256), 0, st, (const U *)x, place, (int)tokens, top, channels, per, (U *)xs)
+    if (dtype == NSPARSE_LM_F32) NSP_GO(unsigned);
     else NSP_GO(unsigned short);
 #undef NSP_GO
     return launched("gather_tokens");
@@ -342,15 +367,14 @@ int nsparse_lm_combine_tokens(int dtype, const void *y, const int *place, const 
     if (tokens == 0) return 0;
     if (!y || !place || !out) return fail(NSPARSE_LM_EARG, "combine_tokens: a required pointer is NULL");
     if (((uintptr_t)y | (uintptr_t)out) % elem_size(dtype)) return fail(NSPARSE_LM_EALIGN, "combine_tokens: y and out begin at elements of their type");
-    const bool wide = (((uintptr_t)y | (uintptr_t)out | (uintptr_t)((long long)channels * elem_size(dtype))) & 15) == 0;
     const int per = threads_per_token(channels, dtype);
     const dim3 grid = groups(ceil_div(tokens, 256 / per));
     hipStream_t st = (hipStream_t)stream;
-#define NSP_GO(T, V) \
-    hipLaunchKernelGGL((k_combine_tokens<T, V>), grid, dim3(256), 0, st, (const T *)y, place, w, (int)tokens, top, channels, per, (T *)out)
-    if (dtype == NSPARSE_LM_BF16) { if (wide) NSP_GO(__bf16, 8); else NSP_GO(__bf16, 1); }
-    else if (dtype == NSPARSE_LM_F16) { if (wide) NSP_GO(_Float16, 8); else NSP_GO(_Float16, 1); }
-    else { if (wide) NSP_GO(float, 4); else NSP_GO(float, 1); }
+#define NSP_GO(T) \
+    hipLaunchKernelGGL(k_combine_tokens<T>, grid, dim3(256), 0, st, (const T *)y, place, w, (int)tokens, top, channels, per, (T *)out)
+    if (dtype == NSPARSE_LM_BF16) NSP_GO(__bf16);
+    else if (dtype == NSPARSE_LM_F16) NSP_GO(_Float16);
+    else NSP_GO(float);
 #undef NSP_GO
     return launched("combine_tokens");
 }
@@ -365,16 +389,15 @@ int nsparse_lm_combine_tokens_bwd(int dtype, const void *dout, const void *y, co
     if (!dout || !place || !dy || (dw && !y) || (w && !dw)) return fail(NSPARSE_LM_EARG, "combine_tokens_bwd: a required pointer is NULL");
     if (((uintptr_t)dout | (uintptr_t)y | (uintptr_t)dy) % elem_size(dtype))
         return fail(NSPARSE_LM_EALIGN, "combine_tokens_bwd: dout, y and dy begin at elements of their type");
-    const bool wide = (((uintptr_t)dout | (uintptr_t)y | (uintptr_t)dy | (uintptr_t)((long long)channels * elem_size(dtype))) & 15) == 0;
     const int per = threads_per_token(channels, dtype);
     const dim3 grid = groups(ceil_div(tokens, 256 / per));
     hipStream_t st = (hipStream_t)stream;
-#define NSP_GO(T, V)                                                                                                                 \
-    hipLaunchKernelGGL((k_combine_tokens_bwd<T, V>), grid, dim3(256), 0, st, (const T *)dout, (const T *)y, place, w, (int)tokens, top, \
+#define NSP_GO(T)                                                                                                                 \
+    hipLaunchKernelGGL(k_combine_tokens_bwd<T>, grid, dim3(256), 0, st, (const T *)dout, (const T *)y, place, w, (int)tokens, top, \
                        channels, per, (T *)dy, dw)
-    if (dtype == NSPARSE_LM_BF16) { if (wide) NSP_GO(__bf16, 8); else NSP_GO(__bf16, 1); }
-    else if (dtype == NSPARSE_LM_F16) { if (wide) NSP_GO(_Float16, 8); else NSP_GO(_Float16, 1); }
-    else { if (wide) NSP_GO(float, 4); else NSP_GO(float, 1); }
+    if (dtype == NSPARSE_LM_BF16) NSP_GO(__bf16);
+    else if (dtype == NSPARSE_LM_F16) NSP_GO(_Float16);
+    else NSP_GO(float);
 #undef NSP_GO
     return launched("combine_tokens_bwd");
 }
