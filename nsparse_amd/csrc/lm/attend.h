@@ -170,7 +170,6 @@ template <int NG, bool WIDE> struct Step {
     int from[kParts], left[kParts];          // first key inside the sequence; keys from there on that some listing query sees
     unsigned long long who[kParts], any;     // queries that list the block
     __device__ inline int first(int y) const { return WIDE ? from[0] + 16 * y : from[y]; }
-    __device__ inline int rows(int y) const { return WIDE ? left[0] - 16 * y : left[y]; }
     __device__ inline unsigned long long lists(int y) const { return who[WIDE ? 0 : y]; }
 };
 template <int NG, bool WIDE> __device__ inline int walk_steps(const Geometry &G, const Union &u)
@@ -252,8 +251,6 @@ template <class T, int DP> struct Columns {
         const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)((const u32x2 *)p1 + (c & 1))));
         return Frag<T>{u32x4{a[0], a[1], b[0], b[1]}};
     }
-    // column of output row 4 quad + e of fragment j, and how many fragments' outputs are neighbours
-    static __device__ inline int column(int j, int quad, int e) { return 16 * j + 4 * quad + e; }
     int q, c;
 };
 template <int DP> struct Columns<float, DP> {
