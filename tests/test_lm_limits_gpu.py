@@ -88,3 +88,38 @@ def test_numbers_that_do_not_fit(lm):
             lm.block_attention(x, x, x, idx, **{"block": 16, **change})
     with pytest.raises(ValueError):
         lm.select_blocks(x, x[:1], block=16, width=2 ** 33, k_rows=4)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+@pytest.mark.parametrize("channels", [1, 7, 8, 37, 1029])
+def test_rows_of_tokens_that_begin_anywhere(lm, dtype, channels):
+    """Tensors whose first element stands behind any multiple of 16 bytes: as tensors that begin at one, and nothing beside them is written."""
+    gen = torch.Generator().manual_seed(channels)
+    T, K, E = 41, 3, 5
+    ids = torch.randint(-1, E, (T, K), generator=gen, dtype=torch.int32).to(DEV)
+    plan = lm.route(ids, E)
+    live = int(plan.offsets[-1])
+    w = torch.rand(T, K, generator=gen).to(DEV)
+
+    def off(t, by):
+        room = torch.full((t.numel() + 32,), 9.0, dtype=t.dtype, device=DEV)
+        room[by:by + t.numel()] = t.flatten()
+        return room[by:by + t.numel()].view(t.shape)
+
+    x, dout = rand(gen, T, channels, dtype=dtype).to(DEV), rand(gen, T, channels, dtype=dtype).to(DEV)
+    xs = lm.gather_tokens(x, plan)
+    y = lm.combine_tokens(xs, plan, w)
+    dy, dw = lm.combine_tokens_backward(dout, xs, plan, w)
+    from nsparse_amd.capi import load_lm
+    for by in (1, 3, 5):
+        assert torch.equal(lm.gather_tokens(off(x, by), plan)[:live], xs[:live])
+        assert torch.equal(lm.combine_tokens(off(xs, by), plan, w), y)
+        a, b = lm.combine_tokens_backward(off(dout, by), off(xs, by), plan, w)
+        assert torch.equal(a[:live], dy[:live]) and torch.equal(b, dw)
+        # an output in the middle of other numbers
+        room = torch.full((T * channels + 32,), 9.0, dtype=dtype, device=DEV)
+        code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+        assert load_lm().nsparse_lm_combine_tokens(code, xs.data_ptr(), plan.place.data_ptr(), w.data_ptr(), T, K, channels,
+                                                   room[by:].data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(room[by:by + T * channels].view(T, channels), y)
+        assert (room[:by] == 9).all() and (room[by + T * channels:] == 9).all()
