@@ -61,7 +61,8 @@ const char *nsparse_lm_build_info(void);
  * row j % page_size of page page_table[s * table_stride + j / page_size].  Query i of a sequence has position
  * len_k - len_q + i; with causal != 0 it attends to keys j <= position, else to all len_k keys.
  * Output rows of queries that no sequence has (behind cu_q[n_seq], or i >= q_len) are left as they were.
- * Numbers in these arrays are clamped to the buffers' sizes; a page outside [0, k_rows) hides its keys.
+ * cu_q and cu_k ascend.  Numbers in these arrays are clamped to the buffers' sizes; where they contradict each other the
+ * results mean nothing, but nothing outside the buffers is read or written.  A page outside [0, k_rows) hides its keys.
  *
  * Pattern.  idx int[q_rows, kv_heads, width]: the blocks (of `block` keys, numbered inside the sequence) that the query's
  * heads of group g attend to.  An entry counts only if it is not negative, lies inside the sequence and is greater

@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
             a++;
             continue;
         }
-        const int z = sq.q_base + sq.q_len < t1 ? (int)(sq.q_base + sq.q_len) : t1;
+        const int z = sq.q_end < t1 ? sq.q_end : t1;
         const Column c0(G, g, slice, per_tile);
         const int col = c0.col, quad = c0.quad;
         // lane i's row for the walk; a column's row is number wave * per_tile + Column::sub
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(256)
             a++;
             continue;
         }
-        const int z = sq.q_base + sq.q_len < t1 ? (int)(sq.q_base + sq.q_len) : t1;
+        const int z = sq.q_end < t1 ? sq.q_end : t1;
         const int t_mine = t0 + lane_id();
         const int limit = t_mine >= a && t_mine < z ? visible_keys(G, sq, (int)(t_mine - sq.q_base)) : 0;
         const int count = z - a;
@@ -203,6 +203,16 @@ __global__ void __launch_bounds__(256)
         }
         a = z;
     }
+}
+
+// Where cu_q does not ascend, words_of_block names words of rows that no sequence or another one has, which k_pattern_bits does not write:
+// they have to be nothing.
+__global__ void __launch_bounds__(256) k_clear_bits(unsigned long long *__restrict__ bits, long long n)
+{
+    const long long x0 = (long long)group_id() * 1024 + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (x0 + 256 * i < n) bits[x0 + 256 * i] = 0;
 }
 
 // The words that can name rows which see block b of a sequence.
@@ -685,6 +695,9 @@ static void launch_bwd(const Geometry &G, const void *q, const void *k, const vo
         if (G.block >= 32) NSP_GO(true); else NSP_GO(false);
 #undef NSP_GO
         if (sp.gms > 0) {
+            // a single sequence's rows are the same to both whatever cu_q holds, and without cu_q they are fixed
+            if (G.cu_q && G.n_seq > 1)
+                hipLaunchKernelGGL(k_clear_bits, groups(ceil_div(sp.gms * sp.words, 1024)), dim3(256), 0, st, bits, sp.gms * sp.words);
             hipLaunchKernelGGL(k_pattern_bits, groups((long long)sp.words * G.kv_heads), dim3(256), 0, st, G, idx, bits, sp.words);
             if (sp.shared_out) {
                 int *counts = (int *)(ws + sp.counts_at);

@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
             a++;
             continue;
         }
-        const int z = sq.q_base + sq.q_len < t1 ? (int)(sq.q_base + sq.q_len) : t1;
+        const int z = sq.q_end < t1 ? sq.q_end : t1;
         const Column c0(G, g, slice, per_tile);
         const int col = c0.col, quad = c0.quad;
         // lane i's row for the walk; a column's row is number (wave * NT + x) * per_tile + Column::sub

@@ -272,6 +272,7 @@ int geometry(const nsparse_lm_attn *a, bool needs_q, bool needs_k, Geometry *g);
 struct Seq {
     int s;            // sequence
     int q_len, k_len; // rows that count
+    int q_end;        // of a query row's sequence: from that row up to here every row is the sequence's
     long long q_base; // first query row
     long long k_base; // first key row (not paged)
 };
@@ -282,6 +283,7 @@ __device__ inline Seq seq_at(const Geometry &G, int s)
 {
     Seq q;
     q.s = s;
+    q.q_end = 0;
     if (G.cu_q) {
         const int a = clampi(G.cu_q[s], 0, G.q_rows), b = clampi(G.cu_q[s + 1], a, G.q_rows);
         q.q_base = a;
@@ -315,22 +317,31 @@ constexpr long long kGridX = 1 << 21, kMostGroups = 0x7fffffffLL - kGridX;
 inline dim3 groups(long long n) { return n <= kGridX ? dim3((unsigned)n) : dim3((unsigned)kGridX, (unsigned)ceil_div(n, kGridX)); }
 __device__ inline unsigned group_id() { return blockIdx.y * gridDim.x + blockIdx.x; }
 
-// the sequence of query row t and the row's number inside it, or -1 where no sequence has it
+// the sequence of query row t and the row's number inside it, or -1 where no sequence has it.  Where cu_q does not ascend the search still
+// decides whose a row is: a number that it finds above t ends the rows that it decides alike.
 __device__ inline int seq_of_query(const Geometry &G, int t, Seq &q)
 {
-    int s;
+    int s, end = G.q_rows;
     if (G.cu_q) {
-        if (t >= G.cu_q[G.n_seq] || t < G.cu_q[0]) return -1;
+        const int last = G.cu_q[G.n_seq];
+        if (t >= last || t < G.cu_q[0]) return -1;
+        end = last < end ? last : end;
         int lo = 0, hi = G.n_seq;  // the last s with cu_q[s] <= t
         while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (G.cu_q[mid] <= t) lo = mid; else hi = mid;
+            const int mid = (lo + hi) >> 1, c = G.cu_q[mid];
+            if (c <= t) {
+                lo = mid;
+            } else {
+                hi = mid;
+                end = c < end ? c : end;
+            }
         }
         s = lo;
     } else {
         s = t / G.q_each;
     }
     q = seq_at(G, s);
+    q.q_end = q.q_base + q.q_len < end ? (int)(q.q_base + q.q_len) : end;
     const long long i = (long long)t - q.q_base;
     return (i >= 0 && i < q.q_len) ? (int)i : -1;
 }
