@@ -627,6 +627,7 @@ int nsparse_lm_block_means(const nsparse_lm_attn *a, const void *k, void *means,
     long long per_seq = 0, rows;
     if (last > 0) per_seq = (last - 1) / G.block + 2;
     if (G.page_size > 0 && (per_seq == 0 || per_seq > G.table_stride * G.per_page)) per_seq = G.table_stride * G.per_page;
+    if (G.page_size > 0 && per_seq == 0) return 0;  // tables without an entry
     rows = per_seq > 0 ? per_seq * G.n_seq : nsparse_lm_mean_rows(a);
     if (rows * G.kv_heads > kMostGroups) return fail(NSPARSE_LM_EARG, "block_means: blocks x heads out of range");
     if (rows == 0) return 0;

@@ -1,0 +1,11 @@
+"""Calls of include/nsparse_lm.h at the edges of their sizes, as far as the host decides: what has nothing to do launches nothing."""
+import ctypes as C
+
+from test_lm_cpu import P, _good, lib  # noqa: F401
+
+
+def test_means_of_a_cache_whose_sequences_have_no_pages(lib):
+    """No table entry, so no block: nothing is launched (a launch would fail here without a GPU, and on one read numbers of no sequence)."""
+    for last in (0, 1, 100):
+        a = _good(page_size=16, k_len=P, page_table=P, table_stride=0, q_rows=1)
+        assert lib.nsparse_lm_block_means(C.byref(a), P, P, last, None) == 0, lib.nsparse_lm_last_error_string()
