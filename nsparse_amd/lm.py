@@ -264,7 +264,10 @@ class _BlockAttention(torch.autograd.Function):
     def backward(ctx, dout, _):
         q, k, v, idx, out, lse = ctx.saved_tensors[:6]
         block, scale, causal, seqs = ctx.rest
-        dq, dk, dv = block_attention_backward(dout.contiguous(), q, k, v, idx, out, lse, block=block, scale=scale, causal=causal, seqs=seqs)
+        dout = dout.contiguous()
+        if dout.data_ptr() % 16:  # a piece of a larger gradient may begin anywhere
+            dout = dout.clone()
+        dq, dk, dv = block_attention_backward(dout, q, k, v, idx, out, lse, block=block, scale=scale, causal=causal, seqs=seqs)
         return dq, dk, dv, None, None, None, None, None
 
 
