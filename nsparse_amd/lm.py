@@ -7,7 +7,8 @@
 Tensors live on one GPU; work is queued on that device's current stream and nothing synchronises, so every call may be captured
 into a graph.  A backward pass is captured by calling the *_backward functions, or through autograd while no graph made outside of the
 capture over the same leaves is alive (refused with RuntimeError where such a graph came from these functions).  Refused
-arguments raise ValueError with the reason.  There is no fallback: a missing library raises.
+arguments raise ValueError with the reason, tensors with a tangent (forward mode) NotImplementedError.  Block means, and so the selection,
+have no derivative: they come without a graph.  There is no fallback: a missing library raises.
 """
 import ctypes as C
 import math
@@ -15,6 +16,7 @@ import struct
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 
 from .capi import LmAttn, load_lm
 
@@ -78,6 +80,12 @@ def _on_gpu(*tensors):
         if t.get_device() != dev:
             raise ValueError("all tensors must live on one device")
     return dev
+
+
+def _no_tangent(*tensors):
+    """Forward mode is refused: a kernel reads a tensor's address, the tangent would be lost."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("there is no derivative in forward mode")
 
 
 def _queued(dev, fn, *args):
@@ -279,6 +287,7 @@ def block_attention(q, k, v, idx, *, block, scale=None, causal=True, seqs=None, 
     """
     seqs = seqs or _ONE
     dev = _on_gpu(q, k, v, idx, *seqs._tensors(), *[t for t in (out, lse) if t is not None])
+    _no_tangent(q, k, v)
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         if out is not None or lse is not None:
@@ -295,6 +304,7 @@ def block_attention_backward(dout, q, k, v, idx, out, lse, *, block, scale=None,
     """(dq, dk, dv) of block_attention from its output and log-sum-exp."""
     seqs = seqs or _ONE
     dev = _on_gpu(dout, q, k, v, idx, out, lse, *seqs._tensors())
+    _no_tangent(dout, q, k, v, out, lse)
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
     a, kv_heads = _attn(seqs, block, q=q, k=k, v=v, width=idx.shape[-1] if idx.dim() == 3 else 0, causal=causal, scale=scale)
     shape = q.shape
@@ -409,6 +419,7 @@ class _Combine(torch.autograd.Function):
 
 def gather_tokens(x, plan):
     """xs [tokens * top, channels]: the tokens' rows expert by expert (rows behind offsets[experts] mean nothing).  Differentiable."""
+    _no_tangent(x)
     if torch.is_grad_enabled() and x.requires_grad:
         return _Gather.apply(x, plan)
     return _gather(x, plan)
@@ -416,6 +427,7 @@ def gather_tokens(x, plan):
 
 def gather_tokens_backward(dxs, plan):
     """dx [tokens, channels]: the sum of each token's rows of dxs."""
+    _no_tangent(dxs)
     return _combine(dxs, plan, None)
 
 
@@ -423,6 +435,7 @@ def combine_tokens(y, plan, weights):
     """out [tokens, channels] = sum over a token's entries of weights [tokens, top] (float32) times their rows of y.  Differentiable."""
     if weights is None:
         raise ValueError("weights must be given; a plain sum of a token's rows is gather_tokens_backward")
+    _no_tangent(y, weights)
     if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad):
         return _Combine.apply(y, plan, weights)
     return _combine(y, plan, weights)
@@ -430,6 +443,7 @@ def combine_tokens(y, plan, weights):
 
 def _combine_backward(dout, y, plan, weights, fill):
     dev = _on_gpu(dout, y, plan.place, weights)
+    _no_tangent(dout, y, weights)
     _rows(dout, "dout", plan.tokens)
     _rows(y, "y", plan.tokens * plan.top)
     if y.dtype != dout.dtype or y.shape[1] != dout.shape[1]:
