@@ -110,11 +110,15 @@ int nsparse_lm_select_blocks(const nsparse_lm_attn *a, const void *q, const void
 int nsparse_lm_block_attention(const nsparse_lm_attn *a, const void *q, const void *k, const void *v, const int *idx,
                                void *out, float *lse, void *stream);
 /* Gradients; out, lse, dout as the forward laid them out; dq like out; dk, dv [k_rows, kv_heads, head_dim] contiguous, key rows
- * that no query reads get 0, key rows outside every sequence are left as they were.  Not for paged caches. */
+ * that no query reads get 0, key rows outside every sequence are left as they were.  Not for paged caches.  The second form adds what
+ * comes back through lse: dlse float[q_rows, heads], NULL for none; what it holds for a query without a key does not count. */
 long long nsparse_lm_block_attention_bwd_workspace(const nsparse_lm_attn *a);
 int nsparse_lm_block_attention_bwd(const nsparse_lm_attn *a, const void *q, const void *k, const void *v, const int *idx,
                                    const void *out, const float *lse, const void *dout, void *dq, void *dk, void *dv,
                                    void *workspace, long long workspace_bytes, void *stream);
+int nsparse_lm_block_attention_lse_bwd(const nsparse_lm_attn *a, const void *q, const void *k, const void *v, const int *idx,
+                                       const void *out, const float *lse, const void *dout, const float *dlse, void *dq, void *dk,
+                                       void *dv, void *workspace, long long workspace_bytes, void *stream);
 
 /* ---- tokens sorted by expert -----------------------------------------------------------------------------------
  * ids int[tokens, top]: entry e = t * top + j names an expert; ids outside [0, experts) are dropped (padding, experts

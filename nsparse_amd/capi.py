@@ -167,6 +167,7 @@ LM_SIGNATURES = {
     "nsparse_lm_block_attention": (_I, [_P(LmAttn)] + [_V] * 7),
     "nsparse_lm_block_attention_bwd_workspace": (_L, [_P(LmAttn)]),
     "nsparse_lm_block_attention_bwd": (_I, [_P(LmAttn)] + [_V] * 11 + [_L, _V]),
+    "nsparse_lm_block_attention_lse_bwd": (_I, [_P(LmAttn)] + [_V] * 12 + [_L, _V]),
     "nsparse_lm_route_workspace": (_L, [_L, _I, _I]),
     "nsparse_lm_route": (_I, [_V, _L, _I, _I, _V, _V, _V, _V, _L, _V]),
     "nsparse_lm_gather_tokens": (_I, [_I, _V, _V, _L, _I, _I, _V, _V]),

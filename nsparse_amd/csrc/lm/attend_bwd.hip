@@ -1,6 +1,6 @@
 // attend_bwd.hip -- gradient of attention over the listed blocks of keys.
 //
-//   p = exp(s - lse), delta = dout . out, ds = p (dout . v - delta)
+//   p = exp(s - lse), delta = dout . out - dlse, ds = p (dout . v - delta)      (dlse: what comes back through the log-sum-exp)
 //   dq = scale sum_j ds_j k_j          over the keys that the query's row lists: the pattern, one wavefront a row
 //   dk = scale sum_t ds_t q_t, dv = sum_t p_t dout_t    over the queries that list the key's block: the transposed pattern
 //
@@ -17,7 +17,7 @@ namespace lm {
 // As the forward for prompts (attend_fwd.hip): the workgroup's rows are the columns of its products, the union of their blocks goes
 // through LDS.  S^T = K Q^T and dP^T = V dO^T read K and V by rows, dQ^T = K^T dS^T reads K transposed.
 // delta comes from the output as the forward rounded it.  That rounding matters where few keys share the weight, so workgroups with
-// at most kExact keys in their union walk twice and take delta = sum p (dout . v) from the first walk.  In single precision the
+// at most kExact keys in their union walk twice and take sum p (dout . v) from the first walk.  In single precision the
 // probabilities are divided by their sum, which takes the rounding of the log-sum-exp out of them.
 // 32 keys a step and one set of columns a wavefront leave three wavefronts a SIMD, which hide each other's reads of LDS, its
 // bound.  4096 rows of 32 heads of 128, 16 blocks each, bf16, against two sets and 64 keys a step (as the forward has where blocks allow):
@@ -30,8 +30,8 @@ struct RowInfo {  // of a query row and head, for dk and dv
 template <class T, int DP, bool WIDE>
 __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
     k_attend_dq(const Geometry G, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ idx,
-                const T *__restrict__ out, const float *__restrict__ lse, const T *__restrict__ dout, T *__restrict__ dq,
-                RowInfo *__restrict__ info, int slices, int per_tile)
+                const T *__restrict__ out, const float *__restrict__ lse, const T *__restrict__ dout, const float *__restrict__ dlse,
+                T *__restrict__ dq, RowInfo *__restrict__ info, int slices, int per_tile)
 {
     constexpr int KS = DP / 32, E = DP / 16, NG = 2 /* groups of sixteen keys a step */, kTile = NG * 16 * Tile<T, DP>::kPieces;
     __shared__ u32x4 kt[2][kTile], vt[2][kTile];
@@ -71,8 +71,10 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
 #pragma unroll
         for (int w = 0; w < KS; w++) rounded += frag_dot(gf[w], qf[w]);
         rounded = quads_sum(rounded);
-        row_frags<T, KS, false>(qf, q + (long long)t * G.q_row + (long long)c0.head * G.q_head, quad, D, on);
         const float lse2 = on ? lse[th] * kLog2e : INFINITY;
+        const auto through_lse = [&] { return dlse && on && lse2 != -INFINITY ? dlse[th] : 0.f; };
+        rounded -= through_lse();
+        row_frags<T, KS, false>(qf, q + (long long)t * G.q_row + (long long)c0.head * G.q_head, quad, D, on);
         const int count = z - a;
         const unsigned long long every = (count < 64 ? (1ULL << count) - 1 : ~0ULL) << (a - t0);
         unsigned long long todo = every, now = every;
@@ -140,7 +142,7 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
                     }
                     if (pass == 0) {
                         const float w = quads_sum(with_dp), l = quads_sum(total);
-                        delta = l > 0.f ? w / l : 0.f;
+                        delta = (l > 0.f ? w / l : 0.f) - through_lse();
                         total = 0.f;
                     }
                 }
@@ -681,7 +683,7 @@ static void launch_dkv(const Geometry &G, const void *q, const void *k, const vo
 
 template <class T, int DP>
 static void launch_bwd(const Geometry &G, const void *q, const void *k, const void *v, const int *idx, const void *out, const float *lse,
-                       const void *dout, void *dq, void *dk, void *dv, char *ws, const BwdSpace &sp, hipStream_t st)
+                       const void *dout, const float *dlse, void *dq, void *dk, void *dv, char *ws, const BwdSpace &sp, hipStream_t st)
 {
     RowInfo *info = (RowInfo *)(ws + sp.info_at);
     unsigned long long *bits = (unsigned long long *)(ws + sp.bits_at);
@@ -690,8 +692,8 @@ static void launch_bwd(const Geometry &G, const void *q, const void *k, const vo
         const int per_tile = G.group < 16 ? 16 / G.group : 1;
 #define NSP_GO(WIDE)                                                                                                                     \
     hipLaunchKernelGGL((k_attend_dq<T, DP, WIDE>), groups(ceil_div(G.q_rows, 4 * per_tile) * slices * G.kv_heads), \
-                       dim3(256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx, (const T *)out, lse, (const T *)dout, (T *)dq,    \
-                       info, slices, per_tile)
+                       dim3(256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx, (const T *)out, lse, (const T *)dout, dlse,       \
+                       (T *)dq, info, slices, per_tile)
         if (G.block >= 32) NSP_GO(true); else NSP_GO(false);
 #undef NSP_GO
         if (sp.gms > 0) {
@@ -735,9 +737,9 @@ long long nsparse_lm_block_attention_bwd_workspace(const nsparse_lm_attn *a)
     return bwd_space(G).total;
 }
 
-int nsparse_lm_block_attention_bwd(const nsparse_lm_attn *a, const void *q, const void *k, const void *v, const int *idx, const void *out,
-                                   const float *lse, const void *dout, void *dq, void *dk, void *dv, void *workspace,
-                                   long long workspace_bytes, void *stream)
+int nsparse_lm_block_attention_lse_bwd(const nsparse_lm_attn *a, const void *q, const void *k, const void *v, const int *idx, const void *out,
+                                       const float *lse, const void *dout, const float *dlse, void *dq, void *dk, void *dv, void *workspace,
+                                       long long workspace_bytes, void *stream)
 {
     using namespace nsp::lm;
     clear_error();
@@ -756,13 +758,20 @@ int nsparse_lm_block_attention_bwd(const nsparse_lm_attn *a, const void *q, cons
     hipStream_t st = (hipStream_t)stream;
     char *ws = (char *)workspace;
 #define NSP_DIM(T)                                                                                                  \
-    if (G.head_dim <= 64) launch_bwd<T, 64>(G, q, k, v, idx, out, lse, dout, dq, dk, dv, ws, sp, st);               \
-    else if (G.head_dim <= 128) launch_bwd<T, 128>(G, q, k, v, idx, out, lse, dout, dq, dk, dv, ws, sp, st);        \
-    else launch_bwd<T, 256>(G, q, k, v, idx, out, lse, dout, dq, dk, dv, ws, sp, st)
+    if (G.head_dim <= 64) launch_bwd<T, 64>(G, q, k, v, idx, out, lse, dout, dlse, dq, dk, dv, ws, sp, st);         \
+    else if (G.head_dim <= 128) launch_bwd<T, 128>(G, q, k, v, idx, out, lse, dout, dlse, dq, dk, dv, ws, sp, st);  \
+    else launch_bwd<T, 256>(G, q, k, v, idx, out, lse, dout, dlse, dq, dk, dv, ws, sp, st)
     if (a->dtype == NSPARSE_LM_BF16) { NSP_DIM(__bf16); }
     else if (a->dtype == NSPARSE_LM_F16) { NSP_DIM(_Float16); }
     else { NSP_DIM(float); }
 #undef NSP_DIM
     return launched("block_attention_bwd");
+}
+
+int nsparse_lm_block_attention_bwd(const nsparse_lm_attn *a, const void *q, const void *k, const void *v, const int *idx, const void *out,
+                                   const float *lse, const void *dout, void *dq, void *dk, void *dv, void *workspace,
+                                   long long workspace_bytes, void *stream)
+{
+    return nsparse_lm_block_attention_lse_bwd(a, q, k, v, idx, out, lse, dout, nullptr, dq, dk, dv, workspace, workspace_bytes, stream);
 }
 }

@@ -264,18 +264,19 @@ class _BlockAttention(torch.autograd.Function):
         out, lse = _attention(q.get_device(), q, k, v, idx, block, scale, causal, seqs, None, None)
         ctx.save_for_backward(q, k, v, idx, out, lse, *seqs._tensors())
         ctx.rest = (block, scale, causal, seqs)
-        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, dout, _):
+    def backward(ctx, dout, dlse):
         q, k, v, idx, out, lse = ctx.saved_tensors[:6]
         block, scale, causal, seqs = ctx.rest
-        dout = dout.contiguous()
+        dout = torch.zeros_like(out) if dout is None else dout.contiguous()
         if dout.data_ptr() % 16:  # a piece of a larger gradient may begin anywhere
             dout = dout.clone()
-        dq, dk, dv = block_attention_backward(dout, q, k, v, idx, out, lse, block=block, scale=scale, causal=causal, seqs=seqs)
+        dlse = None if dlse is None else dlse.contiguous()
+        dq, dk, dv = block_attention_backward(dout, q, k, v, idx, out, lse, block=block, scale=scale, causal=causal, seqs=seqs, dlse=dlse)
         return dq, dk, dv, None, None, None, None, None
 
 
@@ -283,7 +284,8 @@ def block_attention(q, k, v, idx, *, block, scale=None, causal=True, seqs=None, 
     """softmax(scale q k^T) v over the keys of the listed blocks; scale defaults to head_dim ** -0.5.
 
     q [rows, heads, head_dim]; k, v [rows, kv_heads, head_dim] or a paged cache; idx int32 [rows, kv_heads, width] as select_blocks
-    returns it.  Differentiable in q, k, v (not over a paged cache).  out, lse: buffers to write into (then not differentiable).
+    returns it.  Differentiable in q, k, v (not over a paged cache), through the output and through the log-sum-exp [rows, heads] that
+    return_lse adds.  out, lse: buffers to write into (then not differentiable).
     """
     seqs = seqs or _ONE
     dev = _on_gpu(q, k, v, idx, *seqs._tensors(), *[t for t in (out, lse) if t is not None])
@@ -300,11 +302,12 @@ def block_attention(q, k, v, idx, *, block, scale=None, causal=True, seqs=None, 
     return (o, s) if return_lse else o
 
 
-def block_attention_backward(dout, q, k, v, idx, out, lse, *, block, scale=None, causal=True, seqs=None):
-    """(dq, dk, dv) of block_attention from its output and log-sum-exp."""
+def block_attention_backward(dout, q, k, v, idx, out, lse, *, block, scale=None, causal=True, seqs=None, dlse=None):
+    """(dq, dk, dv) of block_attention from its output and log-sum-exp; dlse: the log-sum-exp's own gradient, if it has one."""
     seqs = seqs or _ONE
-    dev = _on_gpu(dout, q, k, v, idx, out, lse, *seqs._tensors())
-    _no_tangent(dout, q, k, v, out, lse)
+    some = [] if dlse is None else [dlse]
+    dev = _on_gpu(dout, q, k, v, idx, out, lse, *some, *seqs._tensors())
+    _no_tangent(dout, q, k, v, out, lse, *some)
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
     a, kv_heads = _attn(seqs, block, q=q, k=k, v=v, width=idx.shape[-1] if idx.dim() == 3 else 0, causal=causal, scale=scale)
     shape = q.shape
@@ -312,6 +315,8 @@ def block_attention_backward(dout, q, k, v, idx, out, lse, *, block, scale=None,
     _contiguous(dout, "dout", q.dtype, shape)
     _contiguous(out, "out", q.dtype, shape)
     _contiguous(lse, "lse", torch.float32, shape[:2])
+    if dlse is not None:
+        _contiguous(dlse, "dlse", torch.float32, shape[:2])
     lib = load_lm()
     ref = C.byref(a)
     need = lib.nsparse_lm_block_attention_bwd_workspace(ref)
@@ -322,8 +327,8 @@ def block_attention_backward(dout, q, k, v, idx, out, lse, *, block, scale=None,
     dk = _empty_or_zeros(whole_k, *k.shape, dtype=q.dtype, device=q.device)
     dv = _empty_or_zeros(whole_k, *k.shape, dtype=q.dtype, device=q.device)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _check(_queued(dev, lib.nsparse_lm_block_attention_bwd, ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), idx.data_ptr(), out.data_ptr(),
-                   lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), need))
+    _check(_queued(dev, lib.nsparse_lm_block_attention_lse_bwd, ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), idx.data_ptr(), out.data_ptr(),
+                   lse.data_ptr(), dout.data_ptr(), _ptr(dlse), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), need))
     return dq, dk, dv
 
 
