@@ -369,56 +369,58 @@ def _rows(t, what, rows):
     _contiguous(t, what)
 
 
-def _weights(w, plan):
+def _weights(w, place):
     if w is not None:
-        _contiguous(w, "weights", torch.float32, (plan.tokens, plan.top))
+        _contiguous(w, "weights", torch.float32, place.shape)
 
 
-def _gather(x, plan):
-    dev = _on_gpu(x, plan.place)
-    _rows(x, "x", plan.tokens)
-    xs = torch.empty(plan.tokens * plan.top, x.shape[1], dtype=x.dtype, device=x.device)
-    _check(_queued(dev, load_lm().nsparse_lm_gather_tokens, _DTYPES[x.dtype], x.data_ptr(), plan.place.data_ptr(), plan.tokens, plan.top,
-                   x.shape[1], xs.data_ptr()))
+def _gather(x, place):
+    dev = _on_gpu(x, place)
+    tokens, top = place.shape
+    _rows(x, "x", tokens)
+    xs = torch.empty(tokens * top, x.shape[1], dtype=x.dtype, device=x.device)
+    _check(_queued(dev, load_lm().nsparse_lm_gather_tokens, _DTYPES[x.dtype], x.data_ptr(), place.data_ptr(), tokens, top, x.shape[1],
+                   xs.data_ptr()))
     return xs
 
 
-def _combine(y, plan, weights):
-    dev = _on_gpu(y, plan.place, *([weights] if weights is not None else []))
-    _rows(y, "y", plan.tokens * plan.top)
-    _weights(weights, plan)
-    out = torch.empty(plan.tokens, y.shape[1], dtype=y.dtype, device=y.device)
-    _check(_queued(dev, load_lm().nsparse_lm_combine_tokens, _DTYPES[y.dtype], y.data_ptr(), plan.place.data_ptr(), _ptr(weights), plan.tokens,
-                   plan.top, y.shape[1], out.data_ptr()))
+def _combine(y, place, weights):
+    dev = _on_gpu(y, place, *([weights] if weights is not None else []))
+    tokens, top = place.shape
+    _rows(y, "y", tokens * top)
+    _weights(weights, place)
+    out = torch.empty(tokens, y.shape[1], dtype=y.dtype, device=y.device)
+    _check(_queued(dev, load_lm().nsparse_lm_combine_tokens, _DTYPES[y.dtype], y.data_ptr(), place.data_ptr(), _ptr(weights), tokens, top,
+                   y.shape[1], out.data_ptr()))
     return out
 
 
+# The plan's rows are saved like any tensor that backward reads: torch tells when they were written again in between.
 class _Gather(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, plan):
+    def forward(ctx, x, place):
         _may_capture(ctx, x)
-        ctx.plan = plan
-        return _gather(x, plan)
+        ctx.save_for_backward(place)
+        return _gather(x, place)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dxs):
-        return gather_tokens_backward(dxs.contiguous(), ctx.plan), None
+        _no_tangent(dxs)
+        return _combine(dxs.contiguous(), *ctx.saved_tensors, None), None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, plan, weights):
+    def forward(ctx, y, place, weights):
         _may_capture(ctx, y, weights)
-        ctx.plan = plan
-        ctx.save_for_backward(y, weights)
-        return _combine(y, plan, weights)
+        ctx.save_for_backward(y, place, weights)
+        return _combine(y, place, weights)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        y, weights = ctx.saved_tensors
-        dy, dw = _combine_backward(dout.contiguous(), y, ctx.plan, weights, fill=True)
+        dy, dw = _combine_backward(dout.contiguous(), *ctx.saved_tensors, fill=True)
         return dy, None, dw
 
 
@@ -426,14 +428,14 @@ def gather_tokens(x, plan):
     """xs [tokens * top, channels]: the tokens' rows expert by expert (rows behind offsets[experts] mean nothing).  Differentiable."""
     _no_tangent(x)
     if torch.is_grad_enabled() and x.requires_grad:
-        return _Gather.apply(x, plan)
-    return _gather(x, plan)
+        return _Gather.apply(x, plan.place)
+    return _gather(x, plan.place)
 
 
 def gather_tokens_backward(dxs, plan):
     """dx [tokens, channels]: the sum of each token's rows of dxs."""
     _no_tangent(dxs)
-    return _combine(dxs, plan, None)
+    return _combine(dxs, plan.place, None)
 
 
 def combine_tokens(y, plan, weights):
@@ -442,25 +444,26 @@ def combine_tokens(y, plan, weights):
         raise ValueError("weights must be given; a plain sum of a token's rows is gather_tokens_backward")
     _no_tangent(y, weights)
     if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad):
-        return _Combine.apply(y, plan, weights)
-    return _combine(y, plan, weights)
+        return _Combine.apply(y, plan.place, weights)
+    return _combine(y, plan.place, weights)
 
 
-def _combine_backward(dout, y, plan, weights, fill):
-    dev = _on_gpu(dout, y, plan.place, weights)
+def _combine_backward(dout, y, place, weights, fill):
+    dev = _on_gpu(dout, y, place, weights)
     _no_tangent(dout, y, weights)
-    _rows(dout, "dout", plan.tokens)
-    _rows(y, "y", plan.tokens * plan.top)
+    tokens, top = place.shape
+    _rows(dout, "dout", tokens)
+    _rows(y, "y", tokens * top)
     if y.dtype != dout.dtype or y.shape[1] != dout.shape[1]:
         raise ValueError("dout and y must have one type and number of channels")
-    _weights(weights, plan)
+    _weights(weights, place)
     dy = (torch.zeros_like if fill else torch.empty_like)(y)
     dw = torch.empty_like(weights)
-    _check(_queued(dev, load_lm().nsparse_lm_combine_tokens_bwd, _DTYPES[y.dtype], dout.data_ptr(), y.data_ptr(), plan.place.data_ptr(),
-                   weights.data_ptr(), plan.tokens, plan.top, y.shape[1], dy.data_ptr(), dw.data_ptr()))
+    _check(_queued(dev, load_lm().nsparse_lm_combine_tokens_bwd, _DTYPES[y.dtype], dout.data_ptr(), y.data_ptr(), place.data_ptr(),
+                   weights.data_ptr(), tokens, top, y.shape[1], dy.data_ptr(), dw.data_ptr()))
     return dy, dw
 
 
 def combine_tokens_backward(dout, y, plan, weights):
     """(dy, dw) of combine_tokens; rows of dy behind offsets[experts] mean nothing."""
-    return _combine_backward(dout, y, plan, weights, fill=False)
+    return _combine_backward(dout, y, plan.place, weights, fill=False)

@@ -205,3 +205,15 @@ def test_two_halves_joined_by_their_log_sum_exp(lm):
     within(out, whole["out"], tol_out, every, "out")
     for i, name in enumerate(("dq", "dk", "dv")):
         within(got[i], whole[name], tol[i], every, name)
+
+
+@pytest.mark.parametrize("op", ["gather", "combine"])
+def test_a_plan_written_again_before_backward(lm, op):
+    gen = torch.Generator().manual_seed(86)
+    T, K, E, Ch = 12, 2, 4, 8
+    plan = lm.route(torch.randint(0, E, (T, K), generator=gen, dtype=torch.int32).to(DEV), E)
+    x, w = rand(gen, T * K if op == "combine" else T, Ch).to(DEV).requires_grad_(), torch.rand(T, K, generator=gen).to(DEV)
+    out = lm.gather_tokens(x, plan) if op == "gather" else lm.combine_tokens(x, plan, w)
+    plan.place.fill_(-1)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        out.sum().backward()
