@@ -110,6 +110,14 @@ def _contiguous(t, what, dtype=None, shape=None):
                          (f", of shape {tuple(shape)}" if shape is not None else ""))
 
 
+def _written(*buffers):
+    """The caller's buffers that a kernel writes count as written in place: a graph that saved one of them refuses its backward."""
+    for t in buffers:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("a buffer to write into must not require a gradient")
+        torch.autograd.graph.increment_version(t)
+
+
 # the fields of LmAttn in their order (an int of padding before the 64-bit ones is the struct module's)
 _ATTN = struct.Struct("@11if3q5P8q")
 assert _ATTN.size == C.sizeof(LmAttn)
@@ -186,6 +194,7 @@ def block_means(k, *, block, seqs=None, last=0, out=None):
         out = _empty_or_zeros(whole, *shape, dtype=k.dtype, device=k.device)
     else:
         _contiguous(out, "out", k.dtype, shape)
+        _written(out)
     _check(_queued(dev, lib.nsparse_lm_block_means, ref, k.data_ptr(), out.data_ptr(), int(last)))
     return out
 
@@ -219,6 +228,7 @@ def select_blocks(q, means, *, block, width, k_rows, first=1, local=1, causal=Tr
         out = torch.empty(shape, dtype=torch.int32, device=q.device) if whole else torch.full(shape, -1, dtype=torch.int32, device=q.device)
     else:
         _contiguous(out, "out", torch.int32, shape)
+        _written(out)
     _check(_queued(dev, lib.nsparse_lm_select_blocks, ref, q.data_ptr(), means.data_ptr(), out.data_ptr()))
     return out
 
@@ -232,10 +242,12 @@ def _attention(dev, q, k, v, idx, block, scale, causal, seqs, out, lse):
         out = _empty_or_zeros(whole, *shape, dtype=q.dtype, device=q.device)
     else:
         _contiguous(out, "out", q.dtype, shape)
+        _written(out)
     if lse is None:
         lse = _empty_or_zeros(whole, shape[0], shape[1], dtype=torch.float32, device=q.device)
     else:
         _contiguous(lse, "lse", torch.float32, shape[:2])
+        _written(lse)
     _check(_queued(dev, load_lm().nsparse_lm_block_attention, C.byref(a), q.data_ptr(), k.data_ptr(), v.data_ptr(), idx.data_ptr(),
                    out.data_ptr(), lse.data_ptr()))
     return out, lse

@@ -217,3 +217,40 @@ def test_a_plan_written_again_before_backward(lm, op):
     plan.place.fill_(-1)
     with pytest.raises(RuntimeError, match="inplace operation"):
         out.sum().backward()
+
+
+def test_buffers_written_again_before_backward(lm):
+    """A pattern, a tensor of keys and an output that a later call writes into: the graph that saved them refuses."""
+    leaves, idx, dout, B = small(87, torch.bfloat16)
+    q, k, v = (x.detach() for x in leaves)
+    n = k.shape[0]
+    means = lm.block_means(k, block=B)
+    base = means.clone()  # means as keys of a second, coarser attention
+    few = torch.zeros(n, k.shape[1], 1, dtype=torch.int32, device=DEV)
+    writes = [(lambda: lm.select_blocks(q, means, block=B, width=idx.shape[2], k_rows=n, out=idx), lambda: lm.block_attention(*leaves, idx, block=B)),
+              (lambda: lm.block_means(k, block=B, out=base), lambda: lm.block_attention(leaves[0], base, base, few, block=16, causal=False))]
+    scaled, log = torch.zeros_like(q), torch.zeros(q.shape[:2], device=DEV)
+    writes.append((lambda: lm.block_attention(q, k, v, idx, block=B, out=scaled), lambda: (scaled * leaves[0]).sum()))
+    writes.append((lambda: lm.block_attention(q, k, v, idx, block=B, lse=log), lambda: (log[:, :, None] * leaves[0]).sum()))
+    for write, use in writes:
+        out = use()
+        write()
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            out.sum().backward()
+
+
+def test_buffers_that_require_a_gradient_are_refused(lm):
+    leaves, idx, _, B = small(88, torch.float32)
+    q, k, v = (x.detach() for x in leaves)
+    wants = torch.empty_like(q).requires_grad_()
+    with pytest.raises(ValueError):
+        lm.block_attention(q, k, v, idx, block=B, out=wants)
+    with pytest.raises(ValueError):
+        lm.block_means(k, block=B, out=torch.empty(-(-k.shape[0] // B), *k.shape[1:], device=DEV).requires_grad_())
+    with torch.no_grad():
+        lm.block_attention(q, k, v, idx, block=B, out=wants)
+    assert torch.equal(wants.detach(), lm.block_attention(q, k, v, idx, block=B))
+    with torch.inference_mode():
+        out = torch.empty_like(q)
+        lm.block_attention(q, k, v, idx, block=B, out=out)
+        assert torch.equal(out, wants)
