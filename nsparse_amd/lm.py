@@ -13,6 +13,7 @@ have no derivative: they come without a graph.  There is no fallback: a missing 
 import ctypes as C
 import math
 import struct
+import threading
 import weakref
 
 import torch
@@ -256,6 +257,7 @@ def _attention(dev, q, k, v, idx, block, scale, causal, seqs, out, lse):
 # Autograd nodes that were made outside of a capture and are alive.  A leaf's gradient is accumulated on the stream on which the first
 # of its living nodes was made: a backward pass captured while one of these lives would leave the capture, which ends the process.
 _eager = weakref.WeakSet()
+_eager_lock = threading.RLock()  # a finalizer may make a node while its thread holds it
 
 
 def _may_capture(ctx, *inputs):
@@ -263,10 +265,13 @@ def _may_capture(ctx, *inputs):
     if not ctx.leaves:
         return
     if torch.cuda.is_current_stream_capturing():
-        if any(x in node.leaves for node in list(_eager) for x in ctx.leaves):
+        with _eager_lock:
+            alive = list(_eager)
+        if any(x in node.leaves for node in alive for x in ctx.leaves):
             raise RuntimeError("a graph made outside of this capture over the same leaves is alive: delete its outputs before capturing")
     else:
-        _eager.add(ctx)
+        with _eager_lock:
+            _eager.add(ctx)
 
 
 class _BlockAttention(torch.autograd.Function):
