@@ -256,22 +256,54 @@ def _attention(dev, q, k, v, idx, block, scale, causal, seqs, out, lse):
 
 # Autograd nodes that were made outside of a capture and are alive.  A leaf's gradient is accumulated on the stream on which the first
 # of its living nodes was made: a backward pass captured while one of these lives would leave the capture, which ends the process.
+# Refused are graphs over the call's own leaves, and those made on the default stream, which cannot join a capture, over leaves
+# further back.
 _eager = weakref.WeakSet()
 _eager_lock = threading.RLock()  # a finalizer may make a node while its thread holds it
 
 
+def _leaves_behind(*starts):
+    """Ids of the leaves that these tensors or autograd nodes come from."""
+    leaves, seen, todo = set(), set(), []
+    for x in starts:
+        if not isinstance(x, torch.Tensor):
+            todo.append(x)
+        elif x.requires_grad and x.is_leaf:
+            leaves.add(id(x))
+        elif x.requires_grad:
+            todo.append(x.grad_fn)
+    while todo:
+        node = todo.pop()
+        if node in seen:
+            continue
+        seen.add(node)
+        try:
+            before = [n for n, _ in node.next_functions if n is not None]
+        except RuntimeError:  # another thread's graph has just gone
+            continue
+        if not before and hasattr(node, "variable"):
+            leaves.add(id(node.variable))
+        todo += before
+    return leaves
+
+
 def _may_capture(ctx, *inputs):
-    ctx.leaves = [id(t) for t in inputs if t.requires_grad and t.is_leaf]
-    if not ctx.leaves:
+    wanted = [t for t in inputs if t.requires_grad]
+    if not wanted:
         return
-    if torch.cuda.is_current_stream_capturing():
-        with _eager_lock:
-            alive = list(_eager)
-        if any(x in node.leaves for node in alive for x in ctx.leaves):
-            raise RuntimeError("a graph made outside of this capture over the same leaves is alive: delete its outputs before capturing")
-    else:
+    ctx.leaves = [id(t) for t in wanted if t.is_leaf]
+    ctx.on_default = _raw_stream(wanted[0].get_device()) == 0
+    if not torch.cuda.is_current_stream_capturing():
         with _eager_lock:
             _eager.add(ctx)
+        return
+    with _eager_lock:
+        alive = list(_eager)
+    if not alive:
+        return
+    behind = _leaves_behind(*wanted)
+    if any(x in node.leaves for node in alive for x in ctx.leaves) or behind & _leaves_behind(*[node for node in alive if node.on_default]):
+        raise RuntimeError("a graph made outside of this capture over the same leaves is alive: delete its outputs before capturing")
 
 
 class _BlockAttention(torch.autograd.Function):

@@ -254,3 +254,38 @@ def test_buffers_that_require_a_gradient_are_refused(lm):
         out = torch.empty_like(q)
         lm.block_attention(q, k, v, idx, block=B, out=out)
         assert torch.equal(out, wants)
+
+
+def test_capture_over_leaves_behind_other_operators(lm):
+    """A weight in front of the call: an eager graph over it, made on the default stream, keeps a capture from starting; a deleted one does not."""
+    leaves, idx, dout, B = small(89, torch.bfloat16)
+    q, k, v = (x.detach() for x in leaves)
+    w = torch.ones(1, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+
+    def forward():
+        return lm.block_attention(q * w, k, v, idx, block=B)
+
+    def step():
+        out = forward()
+        return (out.detach(), *torch.autograd.grad(out, [w], dout))
+
+    alive = forward()
+    with pytest.raises(RuntimeError, match="alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            forward()
+    del alive
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    for _ in range(3):
+        q.copy_(rand(torch.Generator().manual_seed(90), *q.shape, dtype=q.dtype))
+        g.replay()
+        torch.cuda.synchronize()
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del want
