@@ -10,6 +10,7 @@ namespace lm {
 namespace {
 thread_local int t_code = 0;
 thread_local char t_text[256] = "";
+thread_local hipError_t t_launch = hipSuccess;
 }  // namespace
 
 int fail(int code, const char *what)
@@ -22,10 +23,17 @@ void clear_error()
 {
     t_code = 0;
     t_text[0] = 0;
+    t_launch = hipSuccess;
+}
+void note_launch(hipError_t e)
+{
+    if (e == hipSuccess) return;
+    (void)hipGetLastError();  // it is returned, so it is nobody else's
+    if (t_launch == hipSuccess) t_launch = e;
 }
 int launched(const char *what)
 {
-    const hipError_t e = hipGetLastError();
+    const hipError_t e = t_launch;
     if (e == hipSuccess) return 0;
     t_code = (int)e;
     snprintf(t_text, sizeof(t_text), "nsparse_lm: %s: %s", what, hipGetErrorString(e));

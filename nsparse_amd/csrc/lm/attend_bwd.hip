@@ -673,11 +673,11 @@ static void launch_dkv(const Geometry &G, const void *q, const void *k, const vo
     f32x4 *slots = (f32x4 *)(ws + sp.slots_at);
     // floor(r * inv / 2^32) = r / group for r < kListed * group <= 2^20: inv is off by less than group / 2^32 of 1 / group
     const unsigned inv = G.group == 1 ? 0 : (unsigned)((0x100000000ULL + G.group - 1) / G.group);
-    hipLaunchKernelGGL((k_attend_dkv<T, DP, KW, KEYS, ROWS>), groups(sp.max_items * sp.parts), dim3(64 * KEYS * ROWS), 0, st, G,
+    launch((k_attend_dkv<T, DP, KW, KEYS, ROWS>), groups(sp.max_items * sp.parts), dim3(64 * KEYS * ROWS), 0, st, G,
                        (const T *)q, (const T *)k, (const T *)v, (const T *)dout, info, bits, items, n_items, slots, (T *)dk, (T *)dv, sp.words,
                        sp.parts, inv);
     if (sp.shared_out)
-        hipLaunchKernelGGL((k_join_dkv<T, DP, KW, KEYS, ROWS>), groups(sp.max_items * sp.parts), dim3(64 * KEYS), 0, st, G, items, n_items,
+        launch((k_join_dkv<T, DP, KW, KEYS, ROWS>), groups(sp.max_items * sp.parts), dim3(64 * KEYS), 0, st, G, items, n_items,
                            slots, (T *)dk, (T *)dv, sp.parts);
 }
 
@@ -691,7 +691,7 @@ static void launch_bwd(const Geometry &G, const void *q, const void *k, const vo
     if (G.q_rows > 0) {
         const int per_tile = G.group < 16 ? 16 / G.group : 1;
 #define NSP_GO(WIDE)                                                                                                                     \
-    hipLaunchKernelGGL((k_attend_dq<T, DP, WIDE>), groups(ceil_div(G.q_rows, 4 * per_tile) * slices * G.kv_heads), \
+    launch((k_attend_dq<T, DP, WIDE>), groups(ceil_div(G.q_rows, 4 * per_tile) * slices * G.kv_heads), \
                        dim3(256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx, (const T *)out, lse, (const T *)dout, dlse,       \
                        (T *)dq, info, slices, per_tile)
         if (G.block >= 32) NSP_GO(true); else NSP_GO(false);
@@ -699,12 +699,12 @@ static void launch_bwd(const Geometry &G, const void *q, const void *k, const vo
         if (sp.gms > 0) {
             // a single sequence's rows are the same to both whatever cu_q holds, and without cu_q they are fixed
             if (G.cu_q && G.n_seq > 1)
-                hipLaunchKernelGGL(k_clear_bits, groups(ceil_div(sp.gms * sp.words, 1024)), dim3(256), 0, st, bits, sp.gms * sp.words);
-            hipLaunchKernelGGL(k_pattern_bits, groups((long long)sp.words * G.kv_heads), dim3(256), 0, st, G, idx, bits, sp.words);
+                launch(k_clear_bits, groups(ceil_div(sp.gms * sp.words, 1024)), dim3(256), 0, st, bits, sp.gms * sp.words);
+            launch(k_pattern_bits, groups((long long)sp.words * G.kv_heads), dim3(256), 0, st, G, idx, bits, sp.words);
             if (sp.shared_out) {
                 int *counts = (int *)(ws + sp.counts_at);
-                hipLaunchKernelGGL(k_count_rows, groups(ceil_div(sp.gms, 4)), dim3(256), 0, st, G, bits, counts, sp.gms, sp.words);
-                hipLaunchKernelGGL(k_plan_items, dim3(1), dim3(1024), 0, st, counts, sp.gms, sp.per_item, (Item *)(ws + sp.items_at), counts + sp.gms);
+                launch(k_count_rows, groups(ceil_div(sp.gms, 4)), dim3(256), 0, st, G, bits, counts, sp.gms, sp.words);
+                launch(k_plan_items, dim3(1), dim3(1024), 0, st, counts, sp.gms, sp.per_item, (Item *)(ws + sp.items_at), counts + sp.gms);
             }
         }
     }

@@ -400,10 +400,10 @@ static void launch_tiles(const Geometry &G, const void *q, const void *k, const 
     const int per_tile = G.group < 16 ? 16 / G.group : 1;
     const dim3 grid = groups(ceil_div(G.q_rows, 4 * NT * per_tile) * slices * G.kv_heads);
     if (NG == 4 || G.block >= 16 * NG)
-        hipLaunchKernelGGL((k_attend_tiles<T, DP, NT, NG, true>), grid, dim3(256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx,
+        launch((k_attend_tiles<T, DP, NT, NG, true>), grid, dim3(256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx,
                            (T *)out, lse, slices, per_tile);
     else if constexpr (NG == 2)
-        hipLaunchKernelGGL((k_attend_tiles<T, DP, NT, NG, false>), grid, dim3(256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx,
+        launch((k_attend_tiles<T, DP, NT, NG, false>), grid, dim3(256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx,
                            (T *)out, lse, slices, per_tile);
 }
 
@@ -434,7 +434,7 @@ static void launch_attend(const Geometry &G, const void *q, const void *k, const
         return;
     }
 #define NSP_GO(FULL, WAVES)                                                                                                          \
-    hipLaunchKernelGGL((k_attend<T, DP, NG, FULL, WAVES>), groups((WAVES > 1 ? rows : ceil_div(G.q_rows, 4) * slices) * G.kv_heads), \
+    launch((k_attend<T, DP, NG, FULL, WAVES>), groups((WAVES > 1 ? rows : ceil_div(G.q_rows, 4) * slices) * G.kv_heads), \
                        dim3(WAVES > 1 ? 64 * WAVES : 256), 0, st, G, (const T *)q, (const T *)k, (const T *)v, idx, (T *)out, lse, slices)
     if (split) {
         constexpr int kSplit = DP * sizeof(T) > 512 ? 4 : 8;  // registers for a row's sums and a step's keys and values

@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <tuple>
+#include <utility>
 
 #include "nsparse_lm.h"
 
@@ -12,7 +14,21 @@ namespace lm {
 // ---- errors: per thread, as codes (a C entry point never throws or aborts) -----------------------------------------
 int fail(int code, const char *what);
 void clear_error();
-int launched(const char *what);  // hipGetLastError as a return code
+void note_launch(hipError_t e);
+int launched(const char *what);  // the first error of this call's launches as a return code
+
+// A launch whose own result counts: what other code left as the thread's last error is neither taken for ours nor taken away.
+template <class... P, size_t... I>
+inline void launch_packed(const void *kernel, dim3 grid, dim3 block, size_t lds, hipStream_t st, std::tuple<P...> args, std::index_sequence<I...>)
+{
+    void *at[] = {(void *)&std::get<I>(args)...};
+    note_launch(hipLaunchKernel(kernel, grid, block, at, lds, st));
+}
+template <class... P, class... A> inline void launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t st, A... args)
+{
+    static_assert(sizeof...(P) == sizeof...(A), "an argument for every parameter");
+    launch_packed((const void *)kernel, grid, block, lds, st, std::tuple<P...>(args...), std::index_sequence_for<P...>());
+}
 
 inline int elem_size(int dtype) { return dtype == NSPARSE_LM_F32 ? 4 : 2; }
 constexpr long long kMostKeys = 0x7fffffffLL - 4096;  // of a sequence: a block's end is an int too

@@ -329,12 +329,12 @@ int nsparse_lm_route(const int *ids, long long tokens, int top, int experts, int
     while ((1 << bits) < experts) bits++;
     const size_t lds = 4 * (size_t)experts + 2 * (size_t)waves * experts;
     if (chunks == 1) {
-        hipLaunchKernelGGL(k_route_place<true>, dim3(1), dim3(64 * waves), lds, st, ids, n, experts, bits, nullptr, nullptr, offsets, order, place);
+        launch(k_route_place<true>, dim3(1), dim3(64 * waves), lds, st, ids, n, experts, bits, nullptr, nullptr, offsets, order, place);
     } else {
         int *counts = (int *)workspace, *total = counts + (long long)chunks * experts;
-        hipLaunchKernelGGL(k_route_count, dim3(chunks), dim3(64 * waves), 4 * (size_t)experts, st, ids, n, experts, counts);
-        hipLaunchKernelGGL(k_route_prefix, dim3(experts), dim3(64), 0, st, counts, total, chunks, experts);
-        hipLaunchKernelGGL(k_route_place<false>, dim3(chunks), dim3(64 * waves), lds, st, ids, n, experts, bits, counts, total, offsets, order, place);
+        launch(k_route_count, dim3(chunks), dim3(64 * waves), 4 * (size_t)experts, st, ids, n, experts, counts);
+        launch(k_route_prefix, dim3(experts), dim3(64), 0, st, counts, total, chunks, experts);
+        launch(k_route_place<false>, dim3(chunks), dim3(64 * waves), lds, st, ids, n, experts, bits, counts, total, offsets, order, place);
     }
     return launched("route");
 }
@@ -351,7 +351,7 @@ int nsparse_lm_gather_tokens(int dtype, const void *x, const int *place, long lo
     const dim3 grid = groups(ceil_div(tokens, 256 / per));
     hipStream_t st = (hipStream_t)stream;
 #define NSP_GO(U) \
-    hipLaunchKernelGGL(k_gather_tokens<U>, grid, dim3(256), 0, st, (const U *)x, place, (int)tokens, top, channels, per, (U *)xs)
+    launch(k_gather_tokens<U>, grid, dim3(256), 0, st, (const U *)x, place, (int)tokens, top, channels, per, (U *)xs)
     if (dtype == NSPARSE_LM_F32) NSP_GO(unsigned);
     else NSP_GO(unsigned short);
 #undef NSP_GO
@@ -371,7 +371,7 @@ int nsparse_lm_combine_tokens(int dtype, const void *y, const int *place, const 
     const dim3 grid = groups(ceil_div(tokens, 256 / per));
     hipStream_t st = (hipStream_t)stream;
 #define NSP_GO(T) \
-    hipLaunchKernelGGL(k_combine_tokens<T>, grid, dim3(256), 0, st, (const T *)y, place, w, (int)tokens, top, channels, per, (T *)out)
+    launch(k_combine_tokens<T>, grid, dim3(256), 0, st, (const T *)y, place, w, (int)tokens, top, channels, per, (T *)out)
     if (dtype == NSPARSE_LM_BF16) NSP_GO(__bf16);
     else if (dtype == NSPARSE_LM_F16) NSP_GO(_Float16);
     else NSP_GO(float);
@@ -393,7 +393,7 @@ int nsparse_lm_combine_tokens_bwd(int dtype, const void *dout, const void *y, co
     const dim3 grid = groups(ceil_div(tokens, 256 / per));
     hipStream_t st = (hipStream_t)stream;
 #define NSP_GO(T)                                                                                                                 \
-    hipLaunchKernelGGL(k_combine_tokens_bwd<T>, grid, dim3(256), 0, st, (const T *)dout, (const T *)y, place, w, (int)tokens, top, \
+    launch(k_combine_tokens_bwd<T>, grid, dim3(256), 0, st, (const T *)dout, (const T *)y, place, w, (int)tokens, top, \
                        channels, per, (T *)dy, dw)
     if (dtype == NSPARSE_LM_BF16) NSP_GO(__bf16);
     else if (dtype == NSPARSE_LM_F16) NSP_GO(_Float16);

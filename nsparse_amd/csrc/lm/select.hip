@@ -575,11 +575,11 @@ static void launch_rows(const Geometry &G, long long blocks, int first, int loca
 {
     const dim3 grid = groups(ceil_div(G.q_rows, 16) * G.kv_heads);
     if (blocks <= 256)
-        hipLaunchKernelGGL((k_select_rows<T, KS, 256>), grid, dim3(256), 0, st, G, first, local, (const T *)q, (const T *)means, idx);
+        launch((k_select_rows<T, KS, 256>), grid, dim3(256), 0, st, G, first, local, (const T *)q, (const T *)means, idx);
     else if (blocks <= 768)
-        hipLaunchKernelGGL((k_select_rows<T, KS, 768>), grid, dim3(256), 0, st, G, first, local, (const T *)q, (const T *)means, idx);
+        launch((k_select_rows<T, KS, 768>), grid, dim3(256), 0, st, G, first, local, (const T *)q, (const T *)means, idx);
     else
-        hipLaunchKernelGGL((k_select_rows<T, KS, 2048>), grid, dim3(256), 0, st, G, first, local, (const T *)q, (const T *)means, idx);
+        launch((k_select_rows<T, KS, 2048>), grid, dim3(256), 0, st, G, first, local, (const T *)q, (const T *)means, idx);
 }
 
 template <class T>
@@ -599,10 +599,10 @@ static void launch_select(const Geometry &G, int first, int local, const void *q
     if (blocks <= kOneCap) {
         // the plain way wants 32 KB
         const size_t lds = blocks <= 8192 ? 8192 * 4 : (size_t)blocks * 4;
-        if (lds > 65536) (void)hipFuncSetAttribute((const void *)k_select_one<T>, hipFuncAttributeMaxDynamicSharedMemorySize, kOneCap * 4);
-        hipLaunchKernelGGL(k_select_one<T>, grid, dim3(1024), lds, st, G, first, local, (const T *)q, (const T *)means, idx);
+        if (lds > 65536) note_launch(hipFuncSetAttribute((const void *)k_select_one<T>, hipFuncAttributeMaxDynamicSharedMemorySize, kOneCap * 4));
+        launch(k_select_one<T>, grid, dim3(1024), lds, st, G, first, local, (const T *)q, (const T *)means, idx);
     } else {
-        hipLaunchKernelGGL(k_select_long<T>, grid, dim3(256), 0, st, G, first, local, (const T *)q, (const T *)means, idx);
+        launch(k_select_long<T>, grid, dim3(256), 0, st, G, first, local, (const T *)q, (const T *)means, idx);
     }
 }
 
@@ -634,11 +634,11 @@ int nsparse_lm_block_means(const nsparse_lm_attn *a, const void *k, void *means,
     const dim3 grid = groups(rows * G.kv_heads);
     hipStream_t st = (hipStream_t)stream;
     if (a->dtype == NSPARSE_LM_BF16)
-        hipLaunchKernelGGL(k_block_means<__bf16>, grid, dim3(256), 0, st, G, (const __bf16 *)k, (__bf16 *)means, last, (int)per_seq);
+        launch(k_block_means<__bf16>, grid, dim3(256), 0, st, G, (const __bf16 *)k, (__bf16 *)means, last, (int)per_seq);
     else if (a->dtype == NSPARSE_LM_F16)
-        hipLaunchKernelGGL(k_block_means<_Float16>, grid, dim3(256), 0, st, G, (const _Float16 *)k, (_Float16 *)means, last, (int)per_seq);
+        launch(k_block_means<_Float16>, grid, dim3(256), 0, st, G, (const _Float16 *)k, (_Float16 *)means, last, (int)per_seq);
     else
-        hipLaunchKernelGGL(k_block_means<float>, grid, dim3(256), 0, st, G, (const float *)k, (float *)means, last, (int)per_seq);
+        launch(k_block_means<float>, grid, dim3(256), 0, st, G, (const float *)k, (float *)means, last, (int)per_seq);
     return launched("block_means");
 }
 
