@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(256)
             a++;
             continue;
         }
-        const int z = sq.q_end < t1 ? sq.q_end : t1;
+        const int z = sq.q_base + sq.q_len < t1 ? (int)(sq.q_base + sq.q_len) : t1;
         const int hi = competition(G, sq, (int)(z - 1 - sq.q_base), first, local).hi;  // the last row's is the greatest
         float n2max = 0.f;
         for (int b0 = first / 16 * 16 + 16 * wave; b0 < hi; b0 += 64) {
