@@ -130,7 +130,8 @@ int nsparse_lm_block_attention_lse_bwd(const nsparse_lm_attn *a, const void *q, 
 long long nsparse_lm_route_workspace(long long tokens, int top, int experts);
 int nsparse_lm_route(const int *ids, long long tokens, int top, int experts, int *offsets, int *order, int *place,
                      void *workspace, long long workspace_bytes, void *stream);
-/* xs[place[t,j], :] = x[t, :]; rows of xs behind the last expert's are left as they were.  x, xs: contiguous rows of `channels`. */
+/* Where a place is read, one outside [0, tokens * top) counts as dropped.
+ * xs[place[t,j], :] = x[t, :]; rows of xs behind the last expert's are left as they were.  x, xs: contiguous rows of `channels`. */
 int nsparse_lm_gather_tokens(int dtype, const void *x, const int *place, long long tokens, int top, int channels, void *xs,
                              void *stream);
 /* out[t, :] = sum_j w[t,j] y[place[t,j], :], dropped entries left out (none left: 0).  w float[tokens, top], or NULL for ones: then this

@@ -189,11 +189,12 @@ __global__ void __launch_bounds__(256)
     const unsigned t = group_id() * (256 / per) + threadIdx.x / per;
     if (t >= (unsigned)tokens) return;
     const int *pl = place + (long long)t * top;
+    const unsigned rows = (unsigned)tokens * top;
     for (int c = ((int)threadIdx.x % per) * Piece<U>::V; c < channels; c += per * Piece<U>::V) {
         const auto v = Piece<U>::load(x + (long long)t * channels + c, channels - c);
         for (int j = 0; j < top; j++) {
             const int p = pl[j];
-            if (p >= 0) Piece<U>::store(xs + (long long)p * channels + c, v, channels - c);
+            if ((unsigned)p < rows) Piece<U>::store(xs + (long long)p * channels + c, v, channels - c);
         }
     }
 }
@@ -207,12 +208,13 @@ __global__ void __launch_bounds__(256)
     const unsigned t = group_id() * (256 / per) + threadIdx.x / per;
     if (t >= (unsigned)tokens) return;
     const long long e0 = (long long)t * top;
+    const unsigned rows = (unsigned)tokens * top;
     for (int c = ((int)threadIdx.x % per) * V; c < channels; c += per * V) {
         float a[V] = {};
 #pragma unroll 4
         for (int j = 0; j < top; j++) {
             const int p = place[e0 + j];
-            if (p < 0) continue;
+            if ((unsigned)p >= rows) continue;
             const auto x = Piece<T>::load(y + (long long)p * channels + c, channels - c);
             const float f = w ? w[e0 + j] : 1.f;
 #pragma unroll
@@ -241,6 +243,7 @@ __global__ void __launch_bounds__(256)
         for (int j = 0; j < J; j++) {
             const bool in = j0 + j < top;
             p[j] = in ? place[e0 + j0 + j] : -1;
+            if ((unsigned)p[j] >= (unsigned)tokens * top) p[j] = -1;
             f[j] = in && w ? w[e0 + j0 + j] : 1.f;
             dot[j] = 0.f;
         }

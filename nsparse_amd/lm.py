@@ -387,6 +387,8 @@ class Route:
     offsets[experts] means nothing), place int32 [tokens, top] (entry -> sorted row, -1 where dropped)."""
 
     def __init__(self, offsets, order, place):
+        if place.dtype != torch.int32 or place.dim() != 2 or not place.is_contiguous():
+            raise ValueError("place must be a contiguous int32 tensor [tokens, top]")
         self.offsets, self.order, self.place = offsets, order, place
         self.tokens, self.top = place.shape
 
