@@ -625,9 +625,11 @@ int nsparse_lm_block_means(const nsparse_lm_attn *a, const void *k, void *means,
         if (a->k_stride[i] % per16 || a->k_stride[i] < 0) return fail(NSPARSE_LM_EALIGN, "k strides must be multiples of 16 bytes");
     if (((uintptr_t)k | (uintptr_t)means) & 15) return fail(NSPARSE_LM_EALIGN, "block_means: k and means begin at multiples of 16 bytes");
     long long per_seq = 0, rows;
+    // the most blocks a sequence can have
+    const long long most = G.page_size > 0 ? G.table_stride * G.per_page : G.cu_k ? ceil_div(G.k_rows, G.block) : G.blocks_each;
+    if (most == 0) return 0;  // tables without an entry
     if (last > 0) per_seq = (last - 1) / G.block + 2;
-    if (G.page_size > 0 && (per_seq == 0 || per_seq > G.table_stride * G.per_page)) per_seq = G.table_stride * G.per_page;
-    if (G.page_size > 0 && per_seq == 0) return 0;  // tables without an entry
+    if (per_seq > most || (G.page_size > 0 && per_seq == 0)) per_seq = most;
     rows = per_seq > 0 ? per_seq * G.n_seq : nsparse_lm_mean_rows(a);
     if (rows * G.kv_heads > kMostGroups) return fail(NSPARSE_LM_EARG, "block_means: blocks x heads out of range");
     if (rows == 0) return 0;
