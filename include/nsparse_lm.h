@@ -85,7 +85,7 @@ typedef struct nsparse_lm_attn {
     int n_seq;
     int page_size;              /* 0, or a multiple of block */
     int first, local;           /* selection: the first and the last eligible blocks always taken; see select_blocks */
-    float scale;                /* of q.k in the softmax; finite */
+    float scale;                /* of q.k in the softmax; at most 2.3e38 */
     long long q_rows, k_rows;   /* a sequence has at most 2^31 - 4097 keys; q_rows x heads is limited alike */
     long long table_stride;     /* entries of page_table a sequence */
     const int *cu_q, *cu_k, *q_len, *k_len, *page_table;

@@ -1,4 +1,6 @@
 // api.cpp -- error channel and the argument checks that the attention entry points share.
+#include <cfloat>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 
@@ -50,7 +52,8 @@ int geometry(const nsparse_lm_attn *a, bool needs_q, bool needs_k, Geometry *g)
     if (a->head_dim < 8 || a->head_dim > 256 || a->head_dim % 8) return fail(NSPARSE_LM_EARG, "head_dim must be a multiple of 8 up to 256");
     if (a->block < 16 || a->block > 256 || (a->block & (a->block - 1))) return fail(NSPARSE_LM_EARG, "block must be 16, 32, 64, 128 or 256");
     if (a->width < 1 || a->width > 256) return fail(NSPARSE_LM_EARG, "width must be 1 .. 256");
-    if (!(a->scale - a->scale == 0.f)) return fail(NSPARSE_LM_EARG, "scale must be a finite number");
+    // the softmax is taken in base 2: the scale times log2 e has to be a number as well
+    if (!(fabsf(a->scale) * 1.4426950408889634f <= FLT_MAX)) return fail(NSPARSE_LM_EARG, "scale must be a finite number, at most 2.3e38");
     if (a->n_seq < 1) return fail(NSPARSE_LM_EARG, "n_seq must be positive");
     if (a->q_rows < 0 || a->q_rows > 0x7fffffffLL / 2 || a->k_rows < 0) return fail(NSPARSE_LM_EARG, "q_rows or k_rows out of range");
     // one workgroup index per (query row, key head, slice of 16 heads)

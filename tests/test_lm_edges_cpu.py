@@ -20,3 +20,10 @@ def test_refused_gradients_with_that_of_the_log_sum_exp(lib):
         assert lib.nsparse_lm_block_attention_lse_bwd(ref, *args, need, None) == -1, bad
     assert lib.nsparse_lm_block_attention_lse_bwd(ref, *[P] * 12, need - 1, None) == -4
     assert lib.nsparse_lm_block_attention_lse_bwd(ref, *[P] * 11, None, need, None) == -4
+
+
+def test_scales_whose_base_2_form_overflows(lib):
+    """Scores are scaled by scale log2 e: where that is infinite, scores of 0 would be no numbers."""
+    size = lambda x: lib.nsparse_lm_block_attention_bwd_workspace(C.byref(_good(scale=x)))
+    assert size(2.3e38) > 0 and size(-2.3e38) > 0 and size(0.0) > 0
+    assert size(2.4e38) == -1 and size(-2.4e38) == -1 and size(3.4e38) == -1
