@@ -45,7 +45,7 @@ class Seqs:
                                        or page_table.stride(1) != 1 and page_table.shape[1] > 1):
             raise ValueError("Seqs: page_table must be an int32 tensor [n, pages] with contiguous rows")
         # a table cut out of a wider one: its rows count as long as they are apart, so the last one has to be there in full
-        if page_table is not None and self.n > 1 and (
+        if page_table is not None and self.n > 1 and page_table.shape[1] > 0 and (
                 page_table.stride(0) < page_table.shape[1] or
                 page_table.storage_offset() + self.n * page_table.stride(0) > page_table.untyped_storage().nbytes() // 4):
             raise ValueError("Seqs: page_table's rows must not overlap, and a cut of a wider table must keep the last row's end")
@@ -56,7 +56,8 @@ class Seqs:
     ptr_cu_k = property(lambda self: 0 if self.cu_k is None else self.cu_k.data_ptr())
     ptr_q_len = property(lambda self: 0 if self.q_len is None else self.q_len.data_ptr())
     ptr_k_len = property(lambda self: 0 if self.k_len is None else self.k_len.data_ptr())
-    ptr_table = property(lambda self: 0 if self.page_table is None else self.page_table.data_ptr())
+    # (a table without columns is not read, but has to be somewhere)
+    ptr_table = property(lambda self: 0 if self.page_table is None else self.page_table.data_ptr() or self.ptr_k_len)
 
     def _tensors(self):
         return [t for t in (self.cu_q, self.cu_k, self.q_len, self.k_len, self.page_table) if t is not None]
@@ -152,10 +153,11 @@ def _attn(seqs, block, *, q=None, k=None, v=None, kv_heads=None, k_rows=None, pa
             raise ValueError("q, k and v must have one head_dim and type")
         if table is not None:
             page_size = shape[1]
+    table_stride = 0 if table is None else table.stride(0) if seqs.n > 1 and table.shape[1] else table.shape[1]
     try:
         packed = _ATTN.pack(
             dtype, heads, kv_heads, dim, int(block), int(width), 1 if causal else 0, seqs.n, page_size, int(first), int(local), scale, q_rows,
-            int(k_rows), 0 if table is None else (table.stride(0) if seqs.n > 1 else table.shape[1]), 0 if q is None else seqs.ptr_cu_q,
+            int(k_rows), table_stride, 0 if q is None else seqs.ptr_cu_q,
             seqs.ptr_cu_k, 0 if q is None else seqs.ptr_q_len, seqs.ptr_k_len, seqs.ptr_table, q0, q1, *ks, *vs)
     except (struct.error, OverflowError) as e:
         raise ValueError(f"an argument is out of range: {e}") from None

@@ -27,3 +27,23 @@ def test_means_of_the_last_keys_of_any_number(lm, last, packed):
                 assert torch.equal(out[base + b], whole[base + b])
             else:
                 assert (out[base + b] == 7).all()
+
+
+@pytest.mark.parametrize("n", [1, 3])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_conversations_without_a_page(lm, dtype, n):
+    """A table of no columns: no keys, so no blocks, outputs of zeros."""
+    gen = torch.Generator().manual_seed(96)
+    G, D, B = 2, 64, 16
+    k, v = (rand(gen, 4, 32, G, D, dtype=dtype).to(DEV) for _ in range(2))
+    q = rand(gen, n, 4, D, dtype=dtype).to(DEV)
+    seqs = lm.Seqs(n, k_len=i32([7] * n).to(DEV), page_table=torch.empty(n, 0, dtype=torch.int32, device=DEV))
+    means = torch.full((8, G, D), 7.0, dtype=dtype, device=DEV)
+    for last in (0, 1):
+        lm.block_means(k, block=B, seqs=seqs, last=last, out=means)
+    assert (means == 7).all()
+    idx = lm.select_blocks(q, means, block=B, width=4, k_rows=4, seqs=seqs)
+    assert (idx == -1).all()
+    for listed in (idx, torch.zeros_like(idx)):
+        out, lse = lm.block_attention(q, k, v, listed, block=B, seqs=seqs, return_lse=True)
+        assert (out == 0).all() and (lse == -math.inf).all()
