@@ -217,8 +217,7 @@ def experiments_lib_dir():
 EXPERIMENT_SWITCHES = ("NSPARSE_TB_LEAN", "NSPARSE_RANKED_DENS", "NSPARSE_FUSED_FORCE", "NSPARSE_FUSED_BIG", "NSPARSE_TWIN_SAMPLE",
                        "NSPARSE_SYM_CURSOR", "NSPARSE_SPMV_SPLIT", "NSPARSE_SPMV_PIPE", "NSPARSE_SPMV_PLAIN", "NSPARSE_SPMV_ABL",
                        "NSPARSE_SPMV_REMAP", "NSPARSE_SPMV_NOREMAP", "NSPARSE_KEYED", "NSPARSE_KEYED_B", "NSPARSE_TILED",
-                       "NSPARSE_HEAVY_FLAT", "NSPARSE_WINDOW_KERNEL", "NSPARSE_FLAT", "NSPARSE_BLK_DESC", "NSPARSE_STREAM_PRIO",
-                       "NSPARSE_PRIO_BINS")
+                       "NSPARSE_HEAVY_FLAT", "NSPARSE_WINDOW_KERNEL", "NSPARSE_FLAT", "NSPARSE_BLK_DESC")
 
 
 def variant_env(env, base=None):
