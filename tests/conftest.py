@@ -12,6 +12,9 @@ GOLDEN = os.path.join(ROOT, "tests", "golden")
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu)")
+    # NCCL_DEBUG=VERSION makes RCCL print its banner ("RCCL version ...") between the lines that tests read from their children's stdout
+    if os.environ.get("NCCL_DEBUG") == "VERSION":
+        os.environ["NCCL_DEBUG"] = "NONE"
 
 
 # GPU tests written in round 4 while the device pool was closed to this repository: they have never run on the
