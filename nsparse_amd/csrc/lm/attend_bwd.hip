@@ -207,23 +207,29 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// Where cu_q does not ascend, words_of_block names words of rows that no sequence or another one has, which k_pattern_bits does not write:
-// they have to be nothing.
-__global__ void __launch_bounds__(256) k_clear_bits(unsigned long long *__restrict__ bits, long long n)
-{
-    const long long x0 = (long long)group_id() * 1024 + threadIdx.x;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (x0 + 256 * i < n) bits[x0 + 256 * i] = 0;
-}
-
-// The words that can name rows which see block b of a sequence.
+// The words that can name rows which see block b of a sequence: k_pattern_bits has written those and no others.
 __device__ inline void words_of_block(const Geometry &G, const Seq &sq, int b, int &w0, int &w1)
 {
     long long i0 = G.causal ? (long long)b * G.block - (sq.k_len - sq.q_len) : 0;
-    if (i0 < 0) i0 = 0;
-    w0 = (int)((sq.q_base + i0) >> 6);
-    w1 = sq.q_len > i0 ? (int)((sq.q_base + sq.q_len - 1) >> 6) + 1 : w0;
+    long long r0 = sq.q_base + (i0 < 0 ? 0 : i0), r1 = sq.q_base + sq.q_len;
+    if (G.cu_q) {
+        // the rows that seq_of_query gives the sequence, by the steps of its search: all of them where cu_q ascends
+        long long lo = G.cu_q[0], hi = G.cu_q[G.n_seq];
+        for (int x = 0, y = G.n_seq; y - x > 1;) {
+            const int mid = (x + y) >> 1, c = G.cu_q[mid];
+            if (mid <= sq.s) {
+                x = mid;
+                lo = c > lo ? c : lo;
+            } else {
+                y = mid;
+                hi = c < hi ? c : hi;
+            }
+        }
+        r0 = lo > r0 ? lo : r0;
+        r1 = hi < r1 ? hi : r1;
+    }
+    w0 = (int)(r0 >> 6);
+    w1 = r1 > r0 ? (int)((r1 - 1) >> 6) + 1 : w0;
 }
 
 // A block's rows are shared out to items of at most `per_item`, all of a block nearly alike.
@@ -697,9 +703,6 @@ static void launch_bwd(const Geometry &G, const void *q, const void *k, const vo
         if (G.block >= 32) NSP_GO(true); else NSP_GO(false);
 #undef NSP_GO
         if (sp.gms > 0) {
-            // a single sequence's rows are the same to both whatever cu_q holds, and without cu_q they are fixed
-            if (G.cu_q && G.n_seq > 1)
-                launch(k_clear_bits, groups(ceil_div(sp.gms * sp.words, 1024)), dim3(256), 0, st, bits, sp.gms * sp.words);
             launch(k_pattern_bits, groups((long long)sp.words * G.kv_heads), dim3(256), 0, st, G, idx, bits, sp.words);
             if (sp.shared_out) {
                 int *counts = (int *)(ws + sp.counts_at);
