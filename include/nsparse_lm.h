@@ -22,7 +22,7 @@
  *   - Results do not depend on timing: no floating-point atomics.
  *   - Sums, softmax statistics and gradients are accumulated in 32 bits (the block means and the scores near a
  *     selection's border in 64) and rounded once; the probabilities and their gradients are rounded to the
- *     inputs' type on the way into the second product.
+ *     inputs' type on the way into the second product, which adds an error of about the outputs' own rounding.
  */
 #ifndef NSPARSE_AMD_NSPARSE_LM_H
 #define NSPARSE_AMD_NSPARSE_LM_H
@@ -74,6 +74,8 @@ const char *nsparse_lm_build_info(void);
  *   paged     page * (page_size / block) + block inside the page       k_rows * page_size / block rows
  *   cu_k      cu_k[s] / block + s + b                                   k_rows / block + n_seq rows
  *   else      s * ceil(k_rows / n_seq / block) + b
+ * Sequences that share a page share its rows: they have to hold the same keys of a block whose mean a call computes (else one of
+ * their means stands there, which one is open).
  */
 typedef struct nsparse_lm_attn {
     int dtype;                  /* of q, k, v, out, dout, dq, dk, dv, means */

@@ -290,7 +290,8 @@ template <class T, int DP> __device__ inline void store_row(T *p, const f32x4 (&
         }
     }
 }
-// 16 bytes a lane from memory to LDS without registers: lane i's land at the wavefront's `to` + 16 i, the wait is the next barrier's.
+// 16 bytes a lane from memory to LDS without registers: lane i's land at the wavefront's `to` + 16 i.  They are there after the next barrier; the
+// compiler waits for them earlier, before a read of the LDS array that they go to, whatever part of it is read.
 // What is not there (behind head_dim, rows that nobody sees) comes from 16 bytes of zeros.
 static __device__ const u32x4 kNothing[1] = {};
 __device__ inline void fetch(u32x4 *to, const void *from, bool there)

@@ -7,7 +7,8 @@
 // The transposed pattern is a bitmap: for every key head and block one bit a query row, built by 64 rows a workgroup in
 // LDS and written as whole words, so it needs no counting, no sort and no atomics on memory, and the order of
 // the sums in dk and dv is the order of the rows, whatever the timing.  p and scale * ds are rounded to the inputs' type for the second
-// products (with the scale, so that half precision overflows no sooner than the gradients themselves do).
+// products, whose operands in 32 bits would run at a seventh of the rate (with the scale, so that half precision overflows no sooner than the
+// gradients themselves do).
 #include "attend.h"
 
 namespace nsp {
@@ -19,8 +20,8 @@ namespace lm {
 // delta comes from the output as the forward rounded it.  That rounding matters where few keys share the weight, so workgroups with
 // at most kExact keys in their union walk twice and take sum p (dout . v) from the first walk.  In single precision the
 // probabilities are divided by their sum, which takes the rounding of the log-sum-exp out of them.
-// 32 keys a step and one set of columns a wavefront leave three wavefronts a SIMD, which hide each other's reads of LDS, its
-// bound.  4096 rows of 32 heads of 128, 16 blocks each, bf16, against two sets and 64 keys a step (as the forward has where blocks allow):
+// 32 keys a step and one set of columns a wavefront leave three wavefronts a SIMD, which hide each other's reads of LDS and the wait for
+// the next tiles that stands before them (attend_fwd.hip), its bounds.  4096 rows of 32 heads of 128, 16 blocks each, bf16, against two sets and 64 keys a step (as the forward has where blocks allow):
 // blocks of 64: 277 against 313 us, of 32: 195 against 318, of 16: 148 against 210.
 constexpr int kExact = 256;
 struct RowInfo {  // of a query row and head, for dk and dv
@@ -301,7 +302,8 @@ __global__ void __launch_bounds__(1024)
 // An item's workgroup owns up to 64 keys of the block: KEYS wavefronts side by side with KW x 16 keys each, as the columns of their
 // products, and ROWS of them one behind the other, each with its own 32 of the (query, head) pairs that list the block.
 // The pairs' rows of q and dout go through LDS (by rows for S = Q K^T and dP = dO V^T, transposed for dK^T = Q^T dS and
-// dV^T = dO^T P), fetched while the 32 before are computed.  Bound by what LDS delivers: the more keys a wavefront, the fewer reads a product.
+// dV^T = dO^T P), fetched while S and dP of the 32 before are computed (the compiler waits for them before the transposed reads).  Bound by what
+// LDS delivers: the more keys a wavefront, the fewer reads a product.
 // 4096 rows of 32 query and 8 key heads of 128, 16 blocks of 64 each, bf16: 228 us, and 22 for the join of the shared-out blocks' sums; the
 // transposed pattern takes 5 us, counting and planning 5 each.  1501 fp32 rows of 6 and 2 heads of 96, 12 blocks of 16 each: 95 and 10 us.
 constexpr int kItems = 1024;

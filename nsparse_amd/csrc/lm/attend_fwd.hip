@@ -7,13 +7,17 @@
 // 4 (l / 16) + i, which, rounded, is already the right operand of O^T = V^T P^T; V is read row by row, E = DP / 16
 // neighbouring columns a lane, and transposed inside the lane (common.h).  The softmax runs over the blocks with
 // a running maximum and sum in 32 bits, in base 2.
+// The probabilities are rounded to the inputs' type for the second product, half a step each, because products of 32-bit operands run at a
+// seventh of the rate (152 against 1107 TFLOP/s); their sum is taken before that.  That error is about as large as the output's own rounding: against 64 bits the outputs
+// are off by 1.1 to 1.4 times (rms) what the rounding of exact outputs alone would leave.  Single precision rounds nothing.
 // Prompts: a workgroup takes several neighbouring rows, 4 NT x (16 / heads of the group) of them, as the columns of the products of its
 // four wavefronts, and walks the union of their blocks (attend.h): a block that neighbours share is read from the L2 cache
-// once, into LDS, while the block before is computed.
+// once, into LDS.  The next block is asked for before this one's products, but the compiler cannot tell the halves of kt and vt apart and waits
+// for it before the first read of LDS: what hides the way to memory is the other workgroup of the compute unit.
 // With few rows (a serving step) eight wavefronts share a row: wavefront w takes every eighth tile of keys and the partial
 // results meet in LDS.
 // Measured, 32 query and 8 key heads of 128, 16 blocks of 64, bf16.  8192 rows of a prompt whose neighbours agree on part of their blocks: 402 us, 311 TFLOP/s
-// over the listed keys; bound by LDS (a wavefront reads as many cycles of operands as its products take) and by blocks that only
+// over the listed keys; bound by that wait, by LDS (a wavefront reads as many cycles of operands as its products take) and by blocks that only
 // some of the workgroup's rows list.  64 conversations, one row each, 32 blocks: 46 us, 4.2 TB/s, bound by memory.  One row: 15 us, bound by latency.
 #include "attend.h"
 

@@ -6,7 +6,8 @@
 
 Tensors live on one GPU; work is queued on that device's current stream and nothing synchronises, so every call may be captured
 into a graph.  A backward pass is captured by calling the *_backward functions, or through autograd while no graph made outside of the
-capture over the same leaves is alive (refused with RuntimeError where such a graph came from these functions).  Refused
+capture over the same leaves is alive (refused with RuntimeError where such a graph came from these functions, over their own inputs or, made
+on the default stream, over leaves behind them).  Refused
 arguments raise ValueError with the reason, tensors with a tangent (forward mode) NotImplementedError.  Block means, and so the selection,
 have no derivative: they come without a graph.  There is no fallback: a missing library raises.
 """
@@ -179,7 +180,8 @@ def _empty_or_zeros(whole, *shape, dtype, device):
 
 # ---- attention over selected blocks ---------------------------------------------------------------------------------------
 def block_means(k, *, block, seqs=None, last=0, out=None):
-    """Mean of every block of `block` keys, in the keys' type: [rows, kv_heads, head_dim], rows as nsparse_lm.h numbers them.
+    """Mean of every block of `block` keys, in the keys' type: [rows, kv_heads, head_dim], rows as nsparse_lm.h numbers them.  Without a
+    derivative.  Sequences that share a page have to hold the same keys of a block that is computed.
 
     out: a buffer kept from earlier calls (a serving cache keeps it beside the keys); last > 0 then refreshes only the
     blocks that hold the last `last` keys of each sequence.
