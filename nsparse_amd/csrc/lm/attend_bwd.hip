@@ -20,13 +20,15 @@ namespace lm {
 // delta comes from the output as the forward rounded it.  That rounding matters where few keys share the weight, so workgroups with
 // at most kExact keys in their union walk twice and take sum p (dout . v) from the first walk.  In single precision the
 // probabilities are divided by their sum, which takes the rounding of the log-sum-exp out of them.
+// A query with a single key (the first of a sequence) has p = 1 and ds = 0 whatever dout is; dout . v and delta differ by their roundings there, so
+// such rows are counted out: dq = 0, and RowInfo tells dk.
 // 32 keys a step and one set of columns a wavefront leave three wavefronts a SIMD, which hide each other's reads of LDS and the wait for
 // the next tiles that stands before them (attend_fwd.hip), its bounds.  4096 rows of 32 heads of 128, 16 blocks each, bf16, against two sets and 64 keys a step (as the forward has where blocks allow):
 // blocks of 64: 277 against 313 us, of 32: 195 against 318, of 16: 148 against 210.
 constexpr int kExact = 256;
 struct RowInfo {  // of a query row and head, for dk and dv
     float lse2, delta, inv;
-    float pad;
+    float single;  // 1: the row has one key, and its ds is 0
 };
 template <class T, int DP, bool WIDE>
 __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
@@ -82,6 +84,7 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
         while (todo) {
             f32x4 o[E];
             float total = 0.f, with_dp = 0.f, delta = rounded;
+            int keys = 0;  // that the column's row sees; 2 stands for more
 #pragma unroll
             for (int j = 0; j < E; j++) o[j] = f32x4{0, 0, 0, 0};
             const int blocks = (read_lane(limit, 63 - __builtin_clzll(now)) + G.block - 1) / G.block;
@@ -117,7 +120,8 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
                                 });
 #pragma unroll
                             for (int y = 0; y < 2; y++) {
-                                const int vis = (st.lists(y) >> num) & 1 ? lim - st.first(y) - 4 * quad : 0;
+                                const int sees = (st.lists(y) >> num) & 1 ? lim - st.first(y) : 0, vis = sees - 4 * quad;
+                                if (pass == 1) keys += clampi(sees, 0, 2);
 #pragma unroll
                                 for (int e = 0; e < 4; e++) {
                                     const float p = e < vis ? pow2(__builtin_fmaf(s[y][e], sl2, -lse2)) : 0.f;
@@ -162,11 +166,12 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1)
                 const float l = quads_sum(total);
                 inv = l > 0.f ? 1.f / l : 1.f;
             }
+            const bool single = keys == 1 && !dlse;
             const int n = wave * per_tile + c1.sub;
             if (c1.live && ((now >> n) & 1)) {
                 const long long at = (long long)(t0 + n) * G.heads + c1.head;
-                store_row<T, DP>(dq + at * D, o, inv, c1.quad, D);
-                if (c1.quad == 0) info[at] = RowInfo{lse2, delta, inv, 0.f};
+                store_row<T, DP>(dq + at * D, o, single ? 0.f : inv, c1.quad, D);
+                if (c1.quad == 0) info[at] = RowInfo{lse2, delta, inv, single ? 1.f : 0.f};
             }
             todo &= ~now;
             now = todo & -todo;
@@ -437,7 +442,7 @@ __global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>:
         auto ask = [&](int step) {
             const int o = opaque(tid), rr = step * kStep + o;
             ri = RowInfo{INFINITY, 0.f, 1.f, 0.f};
-            lim = 0;
+            lim = 0;  // of a row with a single key: negative in LDS
             if (o < kStep && rr < rows) {
                 const int ti = token_of(rr);
                 const long long t = list[ti];
@@ -451,7 +456,7 @@ __global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>:
                 s_lse2[buf][o] = ri.lse2;
                 s_delta[buf][o] = ri.delta * G.scale;
                 if (sizeof(T) == 4) s_inv[buf][o] = ri.inv;
-                s_limit[buf][o] = lim;
+                s_limit[buf][o] = ri.single != 0.f ? -lim : lim;
             }
         };
         auto prepare = [&](int step, int buf) {
@@ -492,9 +497,10 @@ __global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>:
             const int base = 32 * rw;
             if (step * kStep + base < rows) {
                 Frag<T> pf[KW], df[KW];
-                // rows ascend, and so do the keys they see: the first row sees the fewest (rows that are not there see none)
+                // rows ascend, and so do the keys they see: the first row sees the fewest (rows that are not there see none, and one with a single
+                // key, the block's first, comes first too unless the block has no other)
                 const int fewest = uniform(s_limit[buf][base]), last = uniform(s_limit[buf][base + 31]);
-                const bool all = fewest >= keys_end && last >= keys_end;
+                const bool all = fewest >= keys_end && last >= keys_end && keys_end > b * G.block + 1;
 #pragma unroll
                 for (int y = 0; y < 2; y++) {
                     f32x4 s[KW], ds[KW];
@@ -529,9 +535,9 @@ __global__ void __launch_bounds__(64 * KEYS * ROWS, (Dkv<T, DP, KW, KEYS, ROWS>:
                         for (int x = 0; x < KW; x++)
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
-                                const bool on = key0 + 16 * x < li[e];
+                                const bool single = li[e] < 0, on = key0 + 16 * x < (single ? -li[e] : li[e]);
                                 s[x][e] = on ? s[x][e] : 0.f;
-                                ds[x][e] = on ? ds[x][e] : 0.f;
+                                ds[x][e] = on ? (single ? 0.f * ds[x][e] : ds[x][e]) : 0.f;  // what is no number stays so
                             }
                     }
 #pragma unroll
