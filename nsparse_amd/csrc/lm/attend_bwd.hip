@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(1024)
 // The pairs' rows of q and dout go through LDS (by rows for S = Q K^T and dP = dO V^T, transposed for dK^T = Q^T dS and
 // dV^T = dO^T P), fetched while S and dP of the 32 before are computed (the compiler waits for them before the transposed reads).  Bound by what
 // LDS delivers: the more keys a wavefront, the fewer reads a product.
-// 4096 rows of 32 query and 8 key heads of 128, 16 blocks of 64 each, bf16: 228 us, and 22 for the join of the shared-out blocks' sums; the
+// 4096 rows of 32 query and 8 key heads of 128, 16 blocks of 64 each, bf16: 231 us, and 22 for the join of the shared-out blocks' sums; the
 // transposed pattern takes 5 us, counting and planning 5 each.  1501 fp32 rows of 6 and 2 heads of 96, 12 blocks of 16 each: 95 and 10 us.
 constexpr int kItems = 1024;
 constexpr int kListed = 1024;
